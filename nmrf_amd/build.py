@@ -16,7 +16,11 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libnmrf_hip.so")
 OBJDIR = os.path.join(HERE, "build")
 ARCH = "gfx950"
-FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions (v_pk_*_f32, which -O3 forms by itself from scalar and two-wide float code): some of their forms have given
+# wrong results on this chip now and then.  The host pass does not know the feature and
+# says so.
+FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():

@@ -112,7 +112,7 @@ extern "C" int nmrf_cost_volume_f32(const float *f1, const float *f2, int B, int
 // ------------------------------------------------------------------------------------------------
 // A3: Conv1d(G->8)-ReLU-Conv1d(8->16)-ReLU-Conv1d(16->1) along D (k=5, zero pad 2) + softmax.
 // One wave = TWO pixels, lane = disparity bin: the two pixels are the two halves of a packed fp32 FMA
-// (v_pk_fma_f32: each half an IEEE fma, same (channel, tap) order as the scalar form -> same bits), the
+// (two IEEE fmas, one per pixel, same (channel, tap) order as the scalar form -> same bits), the
 // weight is a wave-uniform SGPR broadcast to both halves, so the weights are read in their reference
 // layout and in memory order (s_load_dwordx16), once per two pixels.  Activations go through a
 // wave-private LDS strip [ch][2+64+2] of pixel pairs (zero guard cells realise the padding; one 8-byte

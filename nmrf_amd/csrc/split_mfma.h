@@ -33,7 +33,7 @@ __device__ __forceinline__ f32x16 mfma16h(h16x8 a, h16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// two fp32 -> packed (hi, lo') pairs: v_cvt_pk_f16_f32, 2 v_cvt_f32_f16, v_pk_add_f32, v_pk_mul_f32, v_cvt_pk_f16_f32
+// two fp32 -> packed (hi, lo') pairs: v_cvt_pk_f16_f32, 2 v_cvt_f32_f16, 2 v_sub_f32, 2 v_mul_f32, v_cvt_pk_f16_f32
 __device__ __forceinline__ void split2(f32x2 a, h16x2 &hi, h16x2 &lo) {
     hi = __builtin_convertvector(a, h16x2);
     const f32x2 back = __builtin_convertvector(hi, f32x2);

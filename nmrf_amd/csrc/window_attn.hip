@@ -584,7 +584,7 @@ __global__ __launch_bounds__(64 * NKT * WPB, OCC) void window_attn_fast_kernel(c
             for (int bj = 0; bj < WIN; ++bj) {
                 const int db = hi ? (bj - bt) : (bt - bj);
                 const float *e = tab + (WIN == 4 ? tab_pos(da + WIN - 1, db + WIN - 1) : rrow + db) * 4;
-                f32x2 s0 = {0.f, 0.f}, s1 = {0.f, 0.f};           // two packed accumulators: 16 v_pk_fma_f32 per dot
+                f32x2 s0 = {0.f, 0.f}, s1 = {0.f, 0.f};           // two packed accumulators: 32 fmas per dot
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float4 t = *reinterpret_cast<const float4 *>(e + c * (POSN * 4));
