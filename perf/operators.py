@@ -333,13 +333,12 @@ def _plain_ffn(s):
 # ---- the framework's calls --------------------------------------------------------------------------------------------------------
 def _own_adamw(s):
     from nmrf_amd import ops
-    case, out, coef = s["case"], {}, None
-    if case["clip"]:
-        out["norm"], coef = ops.grad_norm(s["grads"], max_norm=_CLIP)
-    more = {} if case["bits"] == 32 else {"exp_avg_scales": s["m_scales"], "exp_avg_sq_scales": s["v_scales"], "seed": s["seed"]}
-    ops.adamw_step(s["params"], s["grads"], s["ms"], s["vs"], step=s["step"], lr=_LR, betas=(_B1, _B2), eps=_EPS, weight_decay=s["decay"],
-                   grad_scale=coef, **more)
-    out["p"] = s["p"]
+    case = s["case"]
+    if "plan" not in s:                                             # kept beside the moments for the whole training run
+        scales = () if case["bits"] == 32 else (s["m_scales"], s["v_scales"])
+        s["plan"] = ops.AdamWPlan(s["params"], s["ms"], s["vs"], *scales, weight_decay=s["decay"])
+    norm = s["plan"].step(s["grads"], step=s["step"], lr=_LR, betas=(_B1, _B2), eps=_EPS, max_norm=_CLIP if case["clip"] else None, seed=s["seed"])
+    out = {"norm": norm, "p": s["p"]} if case["clip"] else {"p": s["p"]}
     if case["bits"] == 32:
         return {**out, "m": s["m"], "v": s["v"]}
     return {**out, "m": ops.adamw_moment(s["m"], s["m_scale"]), "v": ops.adamw_moment(s["v"], s["v_scale"], squared=True)}
