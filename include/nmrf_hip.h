@@ -40,8 +40,8 @@ const char *nmrf_strerror(int code);
  * in a separate pass when range_flag != NULL; pass NULL when qkv was produced by nmrf_nmp_block16_f32, which range-checks its q_out. */
 int nmrf_range_scan_f32(const float *x, int64_t n, int *range_flag, void *stream);   /* n % 4 == 0, x 16-byte aligned */
 /* ABI version of this header; bumps on any signature change. */
-#define NMRF_ABI_VERSION 27
-#define NMRF_ABI_STR "27"
+#define NMRF_ABI_VERSION 28
+#define NMRF_ABI_STR "28"
 int nmrf_abi_version(void);   /* = NMRF_ABI_VERSION */
 /* "abi<version>-<16 hex digits>": the digits are a hash of every source and header the library was built from (python -m
  * nmrf_amd.build).  The tools library (libnmrf_hip_debug.so) of the same build returns the same string; the binding refuses one that
@@ -514,6 +514,30 @@ int nmrf_seed_taps_bwd_f32(const float *dcost, const int64_t *seeds, int64_t P, 
 int nmrf_warp_corr_concat_bwd_f32(const float *labels, const float *drow, const float *f1, const float *f2, const float *g1,
                                   const float *g2, int B, int H, int W, int N, int Cf, int Cg, int Gr, float *df1, float *df2, float *dg1,
                                   float *dg2, void *stream);
+
+/* ---- Training-block operators: element types of the entry points that take more than fp32 */
+#define NMRF_F32 0
+#define NMRF_BF16 1
+#define NMRF_F16 2
+
+/* One AdamW step over n tensors (torch.optim.AdamW as the reference builds and steps it, main.py:186-245, 413-430; csrc/adamw.hip holds the
+ * formula and the form of 8-bit moments).  HOST arrays of length n: device addresses p, g (element type dtype), m, v (state_bits 32: fp32;
+ * 8: uint8 codes, with fp32 scales m_scale, v_scale of ceil(numel / 256) entries each and a 32-bit random key per tensor), numel (0 allowed);
+ * hyper [n][4] = 1 - lr * weight_decay, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), eps; betas [4] = beta1, 1 - beta1, beta2, 1 - beta2.
+ * grad_scale: DEVICE scalar that multiplies every gradient (out + 1 of nmrf_grad_norm) or NULL.  p, m, v and the scales are updated in place.
+ * The host arrays are read before the call returns.  One parameter address twice: NMRF_EINVAL; other overlaps are the caller's to rule out. */
+int nmrf_adamw_step(int n, const uint64_t *p, const uint64_t *g, const uint64_t *m, const uint64_t *v, const uint64_t *m_scale,
+                    const uint64_t *v_scale, const int64_t *numel, const float *hyper, const uint32_t *key, const float *betas,
+                    int dtype, int state_bits, const float *grad_scale, void *stream);
+/* The values 8-bit moments stand for: code [n], scale [ceil(n / 256)] -> out [n] fp32 (squared != 0: of the second moment).  The
+ * reference keeps its moments in fp32 (torch.optim.AdamW, main.py:186-245). */
+int nmrf_adamw_moment_f32(const uint8_t *code, const float *scale, int64_t n, int squared, float *out, void *stream);
+/* Sums of squares of n gradient tensors (HOST arrays of device addresses and lengths) in 64 bits, one partial per 8 192 elements of a tensor:
+ * parts [sum of ceil(numel / 8192)] doubles, capacity of them available.  First half of clip_grad_norm_ (main.py:413-430). */
+int nmrf_grad_sqsum(int n, const uint64_t *g, const int64_t *numel, int dtype, double *parts, int64_t capacity, void *stream);
+/* out [2] = the norm, sqrt(sum of parts), and the factor min(1, max_norm / (norm + 1e-6)) of clip_grad_norm_ (main.py:413-430).  The sum has
+ * a fixed order; max_norm may be infinite (factor 1). */
+int nmrf_grad_norm(const double *parts, int64_t count, float max_norm, float *out, void *stream);
 
 #ifdef __cplusplus
 }

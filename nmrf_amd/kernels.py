@@ -1483,3 +1483,47 @@ def warp_corr_concat_backward(labels, drow, f1, f2, g1, g2, n, groups=32):
     _lib.check(_lib.load().nmrf_warp_corr_concat_bwd_f32(_p(labels), _p(drow), _p(f1), _p(f2), _p(g1), _p(g2), b, h, w, n, cf, cg, groups,
                                                          *[_p(t) for t in out], _stream()), "warp_corr_concat_bwd")
     return tuple(out)
+
+
+# ---- training-block operators (csrc/adamw.hip): host tables go in by address, see include/nmrf_hip.h ------------------------------------
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}                  # NMRF_F32 / NMRF_BF16 / NMRF_F16
+ADAMW_BLOCK, GRAD_SQSUM_CHUNK = 256, 8192
+
+
+def _raw_stream():
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())            # (torch.cuda.current_stream() builds an object: 2.5 us)
+
+
+def adamw_step(n, p, g, m, v, m_scale, v_scale, numel, hyper, key, betas, dtype, state_bits, grad_scale):
+    """nmrf_adamw_step on the current stream of the current device.  p ... betas: addresses of HOST tables (nmrf_amd.ops.AdamWPlan keeps them);
+    grad_scale: device scalar or None."""
+    _lib.check(_lib.load().nmrf_adamw_step(n, p, g, m, v, m_scale, v_scale, numel, hyper, key, betas, DTYPE_CODE[dtype], state_bits,
+                                           _p(grad_scale), _raw_stream()), "adamw_step")
+
+
+def grad_sqsum(n, g, numel, dtype, parts):
+    """Partial sums of squares of n gradients (host tables by address) into parts (fp64 device tensor)."""
+    _lib.check(_lib.load().nmrf_grad_sqsum(n, g, numel, DTYPE_CODE[dtype], _p(parts), parts.numel(), _raw_stream()), "grad_sqsum")
+
+
+def grad_norm_factor(parts, max_norm):
+    """parts (fp64) -> (norm, min(1, max_norm / (norm + 1e-6))) as two 0-dim device tensors."""
+    _chk(parts, dtype=torch.float64)
+    out = torch.empty(2, device=parts.device, dtype=torch.float32)
+    _lib.check(_lib.load().nmrf_grad_norm(_p(parts), parts.numel(), float(max_norm), _p(out), _raw_stream()), "grad_norm")
+    return out[0], out[1]
+
+
+@_on_device
+def adamw_moment(code, scale, squared=False):
+    """The values 8-bit moments stand for: code uint8 (any shape), scale fp32 [ceil(numel / 256)] -> fp32 of code's shape (squared: the second
+    moment, whose codes hold the square root)."""
+    _chk(code, dtype=torch.uint8)
+    _chk(scale)
+    if code.device != scale.device or scale.numel() != -(-code.numel() // ADAMW_BLOCK):
+        raise _lib.NmrfHipError("adamw_moment: %d codes need %d scales on the same device, got %d" % (
+            code.numel(), -(-code.numel() // ADAMW_BLOCK), scale.numel()))
+    out = torch.empty(code.shape, device=code.device, dtype=torch.float32)
+    if code.numel():
+        _lib.check(_lib.load().nmrf_adamw_moment_f32(_p(code), _p(scale), code.numel(), int(bool(squared)), _p(out), _raw_stream()), "adamw_moment")
+    return out

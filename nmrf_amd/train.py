@@ -16,6 +16,8 @@ without a reducer); one process per GPU, weights replicated, batch sharded as in
 import torch
 import torch.distributed as dist
 
+from .optim import AdamW
+
 # the WHOLE inference, refinement and propagation stages (attention backward kernels, round 5) and the four prediction heads
 SLICE_PREFIXES = ("infer_head.", "infer_score_head.", "refine_head.", "inference.", "refinement.", "dpn.prop_head.", "dpn.propagation.",
                   "dpn.mlp.")                        # + the seed filter (Conv1d x 3 + softmax: the `init` loss)
@@ -29,7 +31,7 @@ def slice_parameters(model):
     return [(name, p) for name, p in model.named_parameters() if name.startswith(SLICE_PREFIXES)]
 
 
-def build_slice_optimizer(model, cfg):
+def build_slice_optimizer(model, cfg, state_bits=None):
     """AdamW with the reference's parameter groups, in the reference's ORDER (build_optimizer, main.py:186-245; an optimizer state dict
     stores its groups by position, so `checkpoint_latest.pth` of either side loads into the other's optimizer) over the parameters the
     gradient graph reaches: plain parameters at BASE_LR / WEIGHT_DECAY; modules named `*sampling_offsets*` (the MSDeformAttn offsets of
@@ -37,7 +39,9 @@ def build_slice_optimizer(model, cfg):
     (`image_encoder.backbone.*`) at BASE_LR x BACKBONE_LR_DECAY / BACKBONE_WEIGHT_DECAY, its bias tables without decay; the
     relative-position tables of the window attention without weight decay.  Parameters outside the gradient graph are frozen
     (requires_grad False: no kernel could fill their .grad); a parameter the caller froze beforehand STAYS frozen and joins no group,
-    as in the reference (main.py:206-207)."""
+    as in the reference (main.py:206-207).
+    state_bits: None -- torch.optim.AdamW; 32 or 8 -- nmrf_amd.optim.AdamW (one HIP step over all tensors, the gradient clipping inside it)
+    with the moments in that many bits."""
     keep = {id(p) for _, p in slice_parameters(model)}
     for p in model.parameters():
         if id(p) not in keep:
@@ -66,7 +70,9 @@ def build_slice_optimizer(model, cfg):
               {"params": trunk, "lr": s.BASE_LR * s.BACKBONE_LR_DECAY, "weight_decay": s.BACKBONE_WEIGHT_DECAY},
               {"params": trunk_tab, "lr": s.BASE_LR * s.BACKBONE_LR_DECAY, "weight_decay": 0.0},
               {"params": enc_tab, "lr": s.BASE_LR, "weight_decay": 0.0}]
-    return torch.optim.AdamW([g for g in groups if g["params"]], weight_decay=s.WEIGHT_DECAY)
+    groups = [g for g in groups if g["params"]]
+    return torch.optim.AdamW(groups, weight_decay=s.WEIGHT_DECAY) if state_bits is None else AdamW(groups, weight_decay=s.WEIGHT_DECAY,
+                                                                                                   state_bits=state_bits)
 
 
 build_optimizer = build_slice_optimizer          # the reference's name (main.py:186): build_optimizer(model, cfg)
@@ -211,8 +217,11 @@ def train_step(model, criterion, optimizer, sample, grad_clip=1.0, group=None, r
         reducer.finish()                                           # buckets reduced while backward ran (OverlappedGradientReducer)
     else:
         allreduce_gradients(params, group)
-    torch.nn.utils.clip_grad_norm_(params, grad_clip)
-    optimizer.step()
+    if isinstance(optimizer, AdamW):
+        optimizer.step(max_norm=grad_clip)
+    else:
+        torch.nn.utils.clip_grad_norm_(params, grad_clip)
+        optimizer.step()
     return float(losses.detach()), {k: float(v.detach()) for k, v in loss_dict.items()}
 
 
