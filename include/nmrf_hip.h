@@ -40,8 +40,8 @@ const char *nmrf_strerror(int code);
  * in a separate pass when range_flag != NULL; pass NULL when qkv was produced by nmrf_nmp_block16_f32, which range-checks its q_out. */
 int nmrf_range_scan_f32(const float *x, int64_t n, int *range_flag, void *stream);   /* n % 4 == 0, x 16-byte aligned */
 /* ABI version of this header; bumps on any signature change. */
-#define NMRF_ABI_VERSION 28
-#define NMRF_ABI_STR "28"
+#define NMRF_ABI_VERSION 29
+#define NMRF_ABI_STR "29"
 int nmrf_abi_version(void);   /* = NMRF_ABI_VERSION */
 /* "abi<version>-<16 hex digits>": the digits are a hash of every source and header the library was built from (python -m
  * nmrf_amd.build).  The tools library (libnmrf_hip_debug.so) of the same build returns the same string; the binding refuses one that
@@ -538,6 +538,27 @@ int nmrf_grad_sqsum(int n, const uint64_t *g, const int64_t *numel, int dtype, d
 /* out [2] = the norm, sqrt(sum of parts), and the factor min(1, max_norm / (norm + 1e-6)) of clip_grad_norm_ (main.py:413-430).  The sum has
  * a fixed order; max_norm may be infinite (factor 1). */
 int nmrf_grad_norm(const double *parts, int64_t count, float max_norm, float *out, void *stream);
+
+/* The norms around a block fused with its gate and residual scale (csrc/residual_norm.hip; pre-norm blocks of the reference add the branch and
+ * normalise for the next one, nmrf/models/NMP.py:337-364, 366-382, with stochastic depth as a gate, nmrf/models/swin.py:228-233, 300-301):
+ *   z = post ? norm(y) * post_w + post_b : y;   out = x + scale_value * scale * act(gate) * z;   h = norm(out) * next_w + next_b  (h != NULL).
+ * x, y, out, h [T, C] of type dtype, C <= 8192; kind 0 LayerNorm, 1 root-mean-square norm; weights, biases and scale [C] (each may be NULL) in
+ * dtype, or in fp32 when params_f32 != 0; gate (may be NULL): T / gate_rows rows of gate_cols (C or 1) values of type dtype, row r reads row
+ * r / gate_rows; gate_act 0 none, 1 sigmoid, 2 tanh.  out and h may not overlap x or y, except out == x. */
+int nmrf_residual_norm(const void *x, const void *y, int64_t T, int C, int dtype, int kind, float eps, const void *gate,
+                       int64_t gate_rows, int gate_cols, int gate_act, float scale_value, const void *scale, int post,
+                       const void *post_w, const void *post_b, const void *next_w, const void *next_b, int params_f32, void *out,
+                       void *h, void *stream);
+/* floats of the workspace of nmrf_residual_norm_bwd (gate_rows = T without a gate); its reference is autograd (main.py:413-430). */
+int nmrf_residual_norm_bwd_size(int64_t T, int C, int64_t gate_rows, int64_t *floats);
+/* Its backward pass (reference: autograd of the blocks, main.py:413-430): d_out, d_h [T, C] (one may be NULL: zero) -> dx, dy [T, C], dgate (the
+ * gate's shape) and d_scale, d_post_w, d_post_b, d_next_w, d_next_b [C] in the parameters' type; NULL: not asked for.  Recomputed from x and y;
+ * sums over rows in a fixed order.  ws: fp32 workspace of at least the size above. */
+int nmrf_residual_norm_bwd(const void *x, const void *y, const void *d_out, const void *d_h, int64_t T, int C, int dtype, int kind,
+                           float eps, const void *gate, int64_t gate_rows, int gate_cols, int gate_act, float scale_value,
+                           const void *scale, int post, const void *post_w, const void *post_b, const void *next_w, int params_f32,
+                           void *dx, void *dy, void *dgate, void *d_scale, void *d_post_w, void *d_post_b, void *d_next_w,
+                           void *d_next_b, float *ws, int64_t ws_floats, void *stream);
 
 #ifdef __cplusplus
 }

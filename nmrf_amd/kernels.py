@@ -2,6 +2,7 @@
 pointers and the CURRENT torch stream.  PyTorch is plumbing here (memory + streams); all arithmetic
 of these ops happens in libnmrf_hip.so.  Every wrapper refuses non-CUDA tensors: there is no
 fallback path."""
+import ctypes
 import functools
 import os
 
@@ -1527,3 +1528,41 @@ def adamw_moment(code, scale, squared=False):
     if code.numel():
         _lib.check(_lib.load().nmrf_adamw_moment_f32(_p(code), _p(scale), code.numel(), int(bool(squared)), _p(out), _raw_stream()), "adamw_moment")
     return out
+
+
+# the norms around a block (csrc/residual_norm.hip).  `spec`: the call's numbers as nmrf_amd.ops.residual_norm has checked them
+class ResidualNormSpec:
+    __slots__ = ("t", "c", "kind", "eps", "gate_rows", "gate_cols", "gate_act", "scale_value", "post", "next", "params_f32")
+
+
+@_on_device
+def residual_norm(x, y, gate, scale, post_w, post_b, next_w, next_b, s):
+    out, h = torch.empty_like(x), (torch.empty_like(x) if s.next else None)
+    _lib.check(_lib.load().nmrf_residual_norm(_p(x), _p(y), s.t, s.c, DTYPE_CODE[x.dtype], s.kind, s.eps, _p(gate), s.gate_rows, s.gate_cols,
+                                              s.gate_act, s.scale_value, _p(scale), s.post, _p(post_w), _p(post_b), _p(next_w), _p(next_b),
+                                              s.params_f32, _p(out), _p(h), _raw_stream()), "residual_norm")
+    return out, h
+
+
+@_on_device
+def residual_norm_backward(x, y, gate, scale, post_w, post_b, next_w, next_b, d_out, d_h, s, want):
+    """-> gradients of (x, y, gate, scale, post_w, post_b, next_w, next_b); want: which of the last six (None elsewhere)."""
+    dx, dy = torch.empty_like(x), torch.empty_like(y)
+    grads = [torch.empty_like(t) if t is not None and w else None for t, w in zip((gate, scale, post_w, post_b, next_w, next_b), want)]
+    if s.t == 0:
+        return [dx, dy] + [None if g is None else g.zero_() for g in grads]
+    if d_h is None:                                                    # (h was not used: its norm's parameters have no share)
+        for i in (4, 5):
+            if grads[i] is not None:
+                grads[i].zero_()
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().nmrf_residual_norm_bwd_size(s.t, s.c, s.gate_rows if gate is not None else s.t, ctypes.byref(size)), "residual_norm_bwd")
+    ws = torch.empty(size.value, device=x.device, dtype=torch.float32)
+    dg, dsc, dpw, dpb, dnw, dnb = (_p(g) for g in grads)
+    if d_h is None:
+        dnw = dnb = None
+    _lib.check(_lib.load().nmrf_residual_norm_bwd(_p(x), _p(y), _p(d_out), _p(d_h), s.t, s.c, DTYPE_CODE[x.dtype], s.kind, s.eps, _p(gate),
+                                                  s.gate_rows, s.gate_cols, s.gate_act, s.scale_value, _p(scale), s.post, _p(post_w), _p(post_b),
+                                                  _p(next_w), s.params_f32, _p(dx), _p(dy), dg, dsc, dpw, dpb, dnw, dnb, _p(ws), ws.numel(),
+                                                  _raw_stream()), "residual_norm_bwd")
+    return [dx, dy] + grads

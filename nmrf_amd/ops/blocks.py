@@ -1,0 +1,119 @@
+"""Operators of a training block as autograd Functions over the HIP kernels: the norms around it with its gate and residual scale
+(csrc/residual_norm.hip).  They stand beside the reference's block tails, x + proj(attn) / x + mlp(norm2(x)) (nmrf/models/NMP.py:337-364),
+their post-norm form (NMP.py:366-382) and stochastic depth (nmrf/models/swin.py:228-233, 300-301)."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import kernels as K
+from .._lib import NmrfHipError
+
+_GATE_ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
+
+
+def check_rows(name, **tensors):
+    """One device, one type of fp32 / bf16 / fp16, on the GPU; -> that type."""
+    ref = None
+    for k, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise NmrfHipError("%s runs on the MI355X only: %s is a %s tensor (no CPU fallback exists by design)" % (name, k, t.device))
+        if ref is None:
+            ref = t
+            if t.dtype not in K.DTYPE_CODE:
+                raise NmrfHipError("%s: %s is fp32, bf16 or fp16, got %s" % (name, k, t.dtype))
+        if t.device != ref.device:
+            raise NmrfHipError("%s: tensors live on different devices: %s and %s" % (name, ref.device, t.device))
+        if t.dtype != ref.dtype:
+            raise NmrfHipError("%s: %s is %s, expected %s" % (name, k, t.dtype, ref.dtype))
+    return ref.dtype
+
+
+def refuse_captured_backward(name):
+    """A captured backward pass accumulates into leaves on the stream their first graph was built on; with an eager graph of the same leaves
+    alive that is another stream, and the capture takes the process down.  Forward passes are captured freely."""
+    if torch.cuda.is_current_stream_capturing():
+        raise NmrfHipError("%s: a backward pass is not captured into a graph (capture the forward pass, or run it eagerly)" % name)
+
+
+class ResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, post_w, post_b, next_w, next_b, spec):
+        ctx.save_for_backward(x, y, gate, scale, post_w, post_b, next_w, next_b)
+        ctx.spec = spec
+        ctx.set_materialize_grads(False)
+        out, h = K.residual_norm(x, y, gate, scale, post_w, post_b, next_w, next_b, spec)
+        return (out, h) if spec.next else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_h=None):
+        refuse_captured_backward("residual_norm")
+        saved = ctx.saved_tensors
+        if d_out is None and d_h is None:
+            return (None,) * 9
+        d_out, d_h = (None if d is None else d.contiguous() for d in (d_out, d_h))
+        want = [n and t is not None for n, t in zip(ctx.needs_input_grad[2:8], saved[2:])]
+        return (*K.residual_norm_backward(*saved, d_out, d_h, ctx.spec, want), None)
+
+
+def _gate_layout(x, gate):
+    """(rows that share a gate row, 1 or C) of a gate that broadcasts over x from some dimension on; the gate as rows."""
+    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+    lead, c = x.shape[:-1], x.shape[-1]
+    keep = next((k for k in range(len(lead) + 1) if shape[:k] == tuple(lead[:k]) and all(n == 1 for n in shape[k:-1])), None)
+    if gate.dim() > x.dim() or gate.dim() < 1 or shape[-1] not in (1, c) or keep is None:
+        raise ValueError("residual_norm: a gate of shape %s does not share one row with whole trailing dimensions of %s: its leading dimensions "
+                         "are x's up to some point and 1 behind it, its last one %d or 1" % (tuple(gate.shape), tuple(x.shape), c))
+    rows = 1
+    for n in lead[keep:]:
+        rows *= n
+    return max(rows, 1), shape[-1]
+
+
+def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None, scale=None, kind="layer", eps=1e-5):
+    """out = x + scale * act(gate) * z with z = norm(y) (post_norm) or y, and h = norm(out) for the next block (next_norm): the norms before and
+    after a block, its gate and its residual scale in one pass.  -> (out, h), or out alone without next_norm.
+
+    x, y: [..., C], C <= 8192, fp32 / bf16 / fp16 (copied if not contiguous).  post_norm, next_norm: (weight, bias) of the norm, either of them
+    may be None; kind "layer" or "rms".  gate: broadcasts over x with x's leading dimensions up to some point and 1 behind it -- [..., C] per
+    element, [..., 1] per row, [B, 1, C] or [B, 1, 1] per sample (conditioned blocks, stochastic depth: zeros and 1 / keep) --, through
+    gate_act None, "sigmoid" or "tanh".  scale: a number, or a vector over the channels.  Weights, biases and the scale vector are all in x's
+    type or all in fp32.  Differentiable in every tensor; statistics and sums in fp32, the same bits every run.  The forward pass may be
+    captured into a graph, the backward pass may not (it raises)."""
+    if kind not in ("layer", "rms"):
+        raise ValueError("residual_norm: kind is 'layer' or 'rms', got %r" % (kind,))
+    if gate_act not in _GATE_ACTS:
+        raise ValueError("residual_norm: gate_act is None, 'sigmoid' or 'tanh', got %r" % (gate_act,))
+    if x.shape != y.shape or x.dim() < 1:
+        raise ValueError("residual_norm: x %s and y %s differ" % (tuple(x.shape), tuple(y.shape)))
+    if not eps >= 0:
+        raise ValueError("residual_norm: eps %r" % (eps,))
+    c = x.shape[-1]
+    if not 1 <= c <= 8192:
+        raise ValueError("residual_norm: %d channels are not in 1 ... 8192" % c)
+    post_w, post_b = post_norm if post_norm is not None else (None, None)
+    next_w, next_b = next_norm if next_norm is not None else (None, None)
+    vec = scale if isinstance(scale, torch.Tensor) else None
+    dtype = check_rows("residual_norm", x=x, y=y, gate=gate)
+    s = K.ResidualNormSpec()
+    s.params_f32 = 0
+    params = dict(scale=vec, post_weight=post_w, post_bias=post_b, next_weight=next_w, next_bias=next_b)
+    have = {k: t for k, t in params.items() if t is not None}
+    for k, t in have.items():
+        if tuple(t.shape) != (c,):
+            raise ValueError("residual_norm: %s has shape %s, expected (%d,)" % (k, tuple(t.shape), c))
+        if t.device != x.device or not t.is_contiguous():
+            raise NmrfHipError("residual_norm: %s is not a contiguous tensor on %s" % (k, x.device))
+    kinds = {t.dtype for t in have.values()}
+    if kinds - {dtype, torch.float32} or len(kinds) > 1:
+        raise NmrfHipError("residual_norm: weights, biases and the scale vector are all %s or all torch.float32, got %s" % (dtype, sorted(map(str, kinds))))
+    s.params_f32 = int(bool(kinds) and kinds == {torch.float32})
+    s.c, s.t = c, x.numel() // c
+    s.gate_rows, s.gate_cols = _gate_layout(x, gate) if gate is not None else (1, 1)
+    s.gate_act, s.kind, s.eps = _GATE_ACTS[gate_act], int(kind == "rms"), float(eps)
+    s.scale_value = 1.0 if scale is None or vec is not None else float(scale)
+    s.post, s.next = int(post_norm is not None), int(next_norm is not None)
+    x, y = x.contiguous(), y.contiguous()
+    gate = None if gate is None else gate.contiguous()
+    return ResidualNormFn.apply(x, y, gate, vec, post_w, post_b, next_w, next_b, s)
