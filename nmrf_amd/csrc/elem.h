@@ -34,36 +34,56 @@ template <> struct Quad<_Float16> {
     static __device__ __forceinline__ void put(_Float16 *p, float v) { *p = (_Float16)v; }
 };
 
-// N consecutive values (16 bytes, or one value for rows that 16-byte loads do not fit)
-template <typename T, int N> struct Vec {
-    static_assert(N == 1 || N * sizeof(T) == 16, "one value or 16 bytes");
-    static __device__ __forceinline__ void load(const T *p, float *v) {
-        if constexpr (N == 1) v[0] = Quad<T>::one(p);
-        else if constexpr (sizeof(T) == 4) Quad<T>::load(p, v);
-        else {
-            const uint4 t = *reinterpret_cast<const uint4 *>(p);
-            const unsigned w[4] = {t.x, t.y, t.z, t.w};
+// 16 bytes of values as they lie in memory, at any alignment of the element (gfx950 takes unaligned 16-byte accesses), and their fp32 values.
+// Loads are split from unpacking so that a row can be asked for long before it is used.
+template <typename T> struct Vec16 {
+    static constexpr int N = 16 / sizeof(T);
+    static __device__ __forceinline__ uint4 raw(const T *p) {
+        uint4 t;
+        __builtin_memcpy(&t, p, 16);
+        return t;
+    }
+    static __device__ __forceinline__ void unpack(const uint4 &t, float *v) {
+        const unsigned w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (__is_same(T, __bf16)) {
-                    v[2 * j] = __uint_as_float(w[j] << 16);
-                    v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                } else {
-                    v[2 * j] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[j] & 0xffffu));
-                    v[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[j] >> 16));
-                }
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(w[j]);
+            else if constexpr (__is_same(T, __bf16)) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+                v[2 * j] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[j] & 0xffffu));
+                v[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[j] >> 16));
             }
         }
     }
-    static __device__ __forceinline__ void store(T *p, const float *v) {
-        if constexpr (N == 1) Quad<T>::put(p, v[0]);
-        else if constexpr (sizeof(T) == 4) Quad<T>::store(p, v);
-        else {
-            unsigned w[4];
+    static __device__ __forceinline__ uint4 pack(const float *v) {
+        unsigned w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = __builtin_bit_cast(unsigned short, (T)v[2 * j]) | (unsigned)__builtin_bit_cast(unsigned short, (T)v[2 * j + 1]) << 16;
-            *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[j]);
+            else w[j] = __builtin_bit_cast(unsigned short, (T)v[2 * j]) | (unsigned)__builtin_bit_cast(unsigned short, (T)v[2 * j + 1]) << 16;
         }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ void store(T *p, const float *v) {
+        const uint4 t = pack(v);
+        __builtin_memcpy(p, &t, 16);
+    }
+    // the first n < N values, zeros behind them
+    static __device__ __forceinline__ uint4 raw_part(const T *p, int n) {
+        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < n) {
+                if constexpr (sizeof(T) == 4) w[k] = __builtin_bit_cast(unsigned, p[k]);
+                else w[k / 2] |= (unsigned)__builtin_bit_cast(unsigned short, p[k]) << (16 * (k & 1));
+            }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ void store_part(T *p, const float *v, int n) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < n) p[k] = (T)v[k];
     }
 };

@@ -11,6 +11,11 @@
 // values of out, not from its rounded copy.  The backward pass recomputes that row from x and y -- the same bytes as reading a saved out --
 // and keeps the sums over rows (parameters, group gates) in registers: a block writes one partial row at its end, and one more launch adds the
 // partials in a fixed order.  No atomics: the same bits every run.
+//
+// Measured (kernel time): fp32 [29 952, 128], LayerNorm, scale: forward 11.8 us (61 MB, 5.2 TB/s), backward 19.1 + 5 us (92 MB); bf16 [16 384,
+// 4 096], post norm and a tanh gate per sample: forward 100 us (537 MB, 5.3 TB/s), backward 233 + 13 us (805 MB, 3.5 TB/s: two rows a CU in
+// flight at 222 registers a lane, four sums over 8 waves a row).  Loads a row ahead, no load under a branch (each is waited for before the next:
+// 264 -> 233 us), consecutive rows to a block so that a group's gate is read once (forward 161 -> 105 us).
 #include "common.h"
 #include "elem.h"
 #include <initializer_list>
@@ -28,7 +33,7 @@ struct RnArgs {
     float *parts, *gparts;                       // [gridDim][NPARAM][C], [items][C or 1]
     int64_t T, R;                                // R: rows that share a gate row
     int64_t span, items, chunks, rows_per_item;  // backward: items are (span of rows, chunk of it) pairs
-    int C, gate_mode, gate_act, pf32, pvec, rms, post, next, want;      // want: bit P_* = that gradient is asked for, bit 8: dgate
+    int C, gate_mode, gate_act, pf32, rms, post, next, want;      // want: bit P_* = that gradient is asked for, bit 8: dgate
     float eps, scale_value;
 };
 
@@ -78,44 +83,81 @@ __device__ __forceinline__ float gate_value(float g, int act) {
 }
 __device__ __forceinline__ float gate_slope(float a, int act) { return act == 1 ? a * (1.0f - a) : (act == 2 ? 1.0f - a * a : 1.0f); }
 
-template <typename T, int N, int LPR, int E> struct Row {
-    static constexpr int K = N * E;
+// The lanes' elements against the row: EXACT -- each one a channel (powers of two from 64 on); ANY; TINY -- fewer channels than a 16-byte
+// vector holds.  (Clamped addresses and masks cost half as many instructions again as the arithmetic of a row of 128 channels.)
+enum { EXACT = 0, ANY = 1, TINY = 2 };
+template <typename T, int LPR, int E, int FIT> struct Row {
+    static constexpr int N = Vec16<T>::N, K = N * E;
     int C, lane;
-    __device__ __forceinline__ bool in(int j) const { return (j * LPR + lane) * N < C; }
+    bool tail;                                   // (uniform) the last vector of a row is not whole
+    __device__ __forceinline__ Row(int c, int l) : C(FIT == EXACT ? LPR * K : c), lane(l), tail(FIT != EXACT && c % N != 0) {}
     __device__ __forceinline__ int at(int j) const { return (j * LPR + lane) * N; }
-    __device__ __forceinline__ void load(const void *p, int64_t base, float *v) const {
+    __device__ __forceinline__ bool in(int e) const { return FIT == EXACT || at(e / N) + e % N < C; }
+    // Every lane loads, whatever it holds of the row (a load under a branch is waited for before the next one): a vector that the row's end cuts
+    // short comes from the last N channels and is moved into place by place(), one behind the end from the row's start and is dropped there.
+    __device__ __forceinline__ int from(int j) const { return FIT == EXACT || at(j) + N <= C ? at(j) : (at(j) < C ? C - N : 0); }
+    __device__ __forceinline__ void place(float *v) const {
+        if constexpr (FIT == EXACT) return;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            if (in(j)) Vec<T, N>::load(static_cast<const T *>(p) + base + at(j), v + j * N);
-            else
+            float *x = v + j * N;
+            if (FIT == ANY && tail) {
+                const int m = at(j) < C && at(j) + N > C ? at(j) + N - C : 0;
 #pragma unroll
-                for (int k = 0; k < N; ++k) v[j * N + k] = 0.f;
+                for (int s = N / 2; s > 0; s /= 2)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) x[k] = m & s ? (k + s < N ? x[k + s < N ? k + s : 0] : 0.f) : x[k];
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[k] = at(j) < C ? x[k] : 0.f;
         }
+    }
+    __device__ __forceinline__ void ask(const void *p, int64_t base, uint4 *w) const {
+        const T *q = static_cast<const T *>(p) + base;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if constexpr (FIT == TINY) w[j] = Vec16<T>::raw_part(q, j == 0 && lane == 0 ? C : 0);
+            else w[j] = Vec16<T>::raw(q + from(j));
+        }
+    }
+    __device__ __forceinline__ void take(const uint4 *w, float *v) const {
+#pragma unroll
+        for (int j = 0; j < E; ++j) Vec16<T>::unpack(w[j], v + j * N);
+        place(v);
     }
     __device__ __forceinline__ void store(void *p, int64_t base, const float *v) const {
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (in(j)) Vec<T, N>::store(static_cast<T *>(p) + base + at(j), v + j * N);
-    }
-    // a vector over the channels, in the rows' type or in fp32; `none` where there is none
-    __device__ __forceinline__ void param(const RnArgs &a, const void *p, float none, float *v) const {
-#pragma unroll
         for (int j = 0; j < E; ++j) {
-            const int c = at(j);
-            if (!in(j) || !p) {
+            T *q = static_cast<T *>(p) + base + at(j);
+            if (FIT == EXACT || at(j) + N <= C) Vec16<T>::store(q, v + j * N);
+            else if (tail && at(j) < C) Vec16<T>::store_part(q, v + j * N, C - at(j));
+        }
+    }
+    // a vector over the channels, in the rows' type or in fp32; `none` where there is none, 0 behind the last channel
+    __device__ __forceinline__ void param(const RnArgs &a, const void *p, float none, float *v) const {
+        if (!p) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) v[j * N + k] = in(j) ? none : 0.f;
-            } else if (N > 1 && a.pvec) {
-                if (a.pf32)
+            for (int e = 0; e < K; ++e) v[e] = in(e) ? none : 0.f;
+        } else if (!a.pf32) {
+            uint4 w[E];
+            ask(p, 0, w);
+            take(w, v);
+        } else {
+            const float *q = static_cast<const float *>(p);
 #pragma unroll
-                    for (int k = 0; k < N; k += 4) Quad<float>::load(static_cast<const float *>(p) + c + k, v + j * N + k);
-                else
-                    Vec<T, N>::load(static_cast<const T *>(p) + c, v + j * N);
-            } else {
+            for (int j = 0; j < E; ++j) {
+                if constexpr (FIT == TINY) {
 #pragma unroll
-                for (int k = 0; k < N; ++k)
-                    v[j * N + k] = a.pf32 ? static_cast<const float *>(p)[c + k] : Quad<T>::one(static_cast<const T *>(p) + c + k);
+                    for (int k = 0; k < N; ++k) v[j * N + k] = q[at(j) + k < C ? at(j) + k : 0];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < N; k += 4) Vec16<float>::unpack(Vec16<float>::raw(q + from(j) + k), v + j * N + k);
+                }
             }
+            if (FIT == TINY)
+#pragma unroll
+                for (int e = 0; e < K; ++e) v[e] = in(e) ? v[e] : 0.f;
+            else place(v);
         }
     }
     // v -> (v - mean) * rstd (layer) or v * rstd (rms); returns rstd
@@ -127,7 +169,10 @@ template <typename T, int N, int LPR, int E> struct Row {
             for (int e = 0; e < K; ++e) s += v[e];
             const float mean = rs.one(s) * inv;
 #pragma unroll
-            for (int e = 0; e < K; ++e) v[e] = in(e / N) ? v[e] - mean : 0.f;
+            for (int e = 0; e < K; ++e) v[e] -= mean;
+            if (FIT != EXACT)
+#pragma unroll
+                for (int e = 0; e < K; ++e) v[e] = in(e) ? v[e] : 0.f;
         }
         float q = 0.f;
 #pragma unroll
@@ -151,44 +196,65 @@ template <typename T, int N, int LPR, int E> struct Row {
 #pragma unroll
         for (int e = 0; e < K; ++e) u[e] = rstd * (u[e] - su - vhat[e] * sx);
     }
-    // act(gate) of row r: one value (GV false), or one for each element
-    template <bool GV> __device__ __forceinline__ void gate(const RnArgs &a, int64_t r, float *g) const {
+    // act(gate) of row r, read again only when the row's gate row is another one: one value (GV false), or one for each element
+    template <bool GV> __device__ __forceinline__ void gate(const RnArgs &a, int64_t r, int64_t &held, float *g) const {
+        if (a.gate_mode == GATE_NONE) return;
         const int64_t gr = a.R == 1 ? r : r / a.R;
+        if (gr == held) return;
+        held = gr;
         if constexpr (GV) {
-            load(a.gate, gr * a.C, g);
+            uint4 w[E];
+            ask(a.gate, gr * a.C, w);
+            take(w, g);
 #pragma unroll
             for (int e = 0; e < K; ++e) g[e] = gate_value(g[e], a.gate_act);
         } else {
-            g[0] = a.gate_mode == GATE_NONE ? 1.f : gate_value(Quad<T>::one(static_cast<const T *>(a.gate) + gr), a.gate_act);
+            g[0] = gate_value(Quad<T>::one(static_cast<const T *>(a.gate) + gr), a.gate_act);
         }
     }
 };
 
 template <int LPR> constexpr int rn_threads() { return LPR <= 256 ? 256 : LPR; }
 
-template <typename T, int N, int LPR, int E>
+template <typename T, int LPR, int E, int FIT>
 __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_fwd_kernel(RnArgs a) {
-    constexpr int K = N * E, ROWS = rn_threads<LPR>() / LPR;
+    constexpr int K = Row<T, LPR, E, FIT>::K, ROWS = rn_threads<LPR>() / LPR;
     __shared__ float sh[2][2][8];
     RowSum<LPR> rs{sh};
-    const Row<T, N, LPR, E> row{a.C, (int)(threadIdx.x % LPR)};
-    float pw[K], pb[K], nw[K], nb[K], sc[K];
+    const Row<T, LPR, E, FIT> row(a.C, (int)(threadIdx.x % LPR));
+    const bool gv = a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP;
+    float pw[K], pb[K], nw[K], nb[K], sc[K], g[K];
+    // (a block owns consecutive rows: they share their gate row as long as they can)
+    const int64_t r1 = min(a.T, (int64_t)(blockIdx.x + 1) * a.rows_per_item);
+    int64_t r = (int64_t)blockIdx.x * a.rows_per_item + threadIdx.x / LPR, held = -1;
+    uint4 wx[E], wy[E];
+    if (r < r1) {
+        row.ask(a.y, r * a.C, wy);
+        row.ask(a.x, r * a.C, wx);
+    }
     row.param(a, a.post_w, 1.f, pw);
     row.param(a, a.post_b, 0.f, pb);
     row.param(a, a.next_w, 1.f, nw);
     row.param(a, a.next_b, 0.f, nb);
     row.param(a, a.scale, 1.f, sc);
 #pragma unroll
-    for (int e = 0; e < K; ++e) sc[e] *= a.scale_value;
+    for (int e = 0; e < K; ++e) {
+        sc[e] *= a.scale_value;
+        g[e] = 1.f;
+    }
     // (rows of one wave or less: lanes behind the last row leave; a row of several waves has the whole block's barriers in step)
-    for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR; r < a.T; r += (int64_t)gridDim.x * ROWS) {
-        float x[K], z[K], g[K];
-        row.load(a.y, r * a.C, z);
-        row.load(a.x, r * a.C, x);
-        if (a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP) {
-            row.template gate<true>(a, r, g);
-        } else {
-            row.template gate<false>(a, r, g);
+    for (; r < r1; r += ROWS) {
+        float x[K], z[K];
+        row.take(wy, z);
+        row.take(wx, x);
+        if (r + ROWS < r1) {                                       // the next row is on its way while this one waits for its sums
+            row.ask(a.y, (r + ROWS) * a.C, wy);
+            row.ask(a.x, (r + ROWS) * a.C, wx);
+        }
+        if (gv) {
+            row.template gate<true>(a, r, held, g);
+        } else if (a.gate_mode != GATE_NONE) {
+            row.template gate<false>(a, r, held, g);
 #pragma unroll
             for (int e = 1; e < K; ++e) g[e] = g[0];
         }
@@ -210,9 +276,9 @@ __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_fwd_kernel(Rn
 }
 
 // sum of a lane's K values over the rows a block holds side by side -> dst [C], written by the lanes of its first row
-template <typename T, int N, int LPR, int E>
-__device__ __forceinline__ void block_columns(const Row<T, N, LPR, E> &row, float *v, float *dst) {
-    constexpr int K = N * E;
+template <typename T, int LPR, int E, int FIT>
+__device__ __forceinline__ void block_columns(const Row<T, LPR, E, FIT> &row, float *v, float mul, float *dst) {
+    constexpr int K = Row<T, LPR, E, FIT>::K, N = Row<T, LPR, E, FIT>::N;
     if constexpr (LPR < 64) {
 #pragma unroll
         for (int e = 0; e < K; ++e) {
@@ -236,52 +302,69 @@ __device__ __forceinline__ void block_columns(const Row<T, N, LPR, E> &row, floa
     }
     if (threadIdx.x < LPR)
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (row.in(j))
-#pragma unroll
-                for (int k = 0; k < N; ++k) dst[row.at(j) + k] = v[j * N + k];
+        for (int e = 0; e < K; ++e)
+            if (row.in(e)) dst[row.at(e / N) + e % N] = v[e] * mul;
 }
 
 // GV: the gate is a vector over the channels (one value a row, or none, keeps 2 K registers free)
-template <typename T, int N, int LPR, int E, bool GV>
+template <typename T, int LPR, int E, int FIT, bool GV>
 __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_bwd_kernel(RnArgs a) {
-    constexpr int K = N * E, THREADS = rn_threads<LPR>(), ROWS = THREADS / LPR, GK = GV ? K : 1;
+    constexpr int K = Row<T, LPR, E, FIT>::K, THREADS = rn_threads<LPR>(), ROWS = THREADS / LPR, GK = GV ? K : 1;
     __shared__ float sh[2][2][8];
     __shared__ float ones[THREADS / 64];
     RowSum<LPR> rs{sh};
-    const Row<T, N, LPR, E> row{a.C, (int)(threadIdx.x % LPR)};
-    float pw[K], nw[K], sc[K], acc[NPARAM][K];
+    const Row<T, LPR, E, FIT> row(a.C, (int)(threadIdx.x % LPR));
+    float pw[K], nw[K], sc[K], g[GK], acc[NPARAM][K];
     row.param(a, a.post_w, 1.f, pw);
     row.param(a, a.next_w, 1.f, nw);
     row.param(a, a.scale, 1.f, sc);
 #pragma unroll
+    for (int e = 0; e < K; ++e) sc[e] *= a.scale_value;
+#pragma unroll
+    for (int e = 0; e < GK; ++e) g[e] = 1.f;
+#pragma unroll
     for (int q = 0; q < NPARAM; ++q)
 #pragma unroll
         for (int e = 0; e < K; ++e) acc[q][e] = 0.f;
+    int64_t held = -1;
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t group = item / a.chunks, first = (item - group * a.chunks) * a.rows_per_item;
         const int64_t r1 = group * a.span + (first + a.rows_per_item < a.span ? first + a.rows_per_item : a.span);
         float ga[GK];
 #pragma unroll
         for (int e = 0; e < GK; ++e) ga[e] = 0.f;
-        for (int64_t r = group * a.span + first + threadIdx.x / LPR; r < r1; r += ROWS) {
-            float z[K], t[K], g[GK], d[K], u[K], b[K];
-            row.load(a.y, r * a.C, z);
-            row.load(a.x, r * a.C, t);
-            if (a.d_h) row.load(a.d_h, r * a.C, u);
-            if (a.d_out) row.load(a.d_out, r * a.C, d);
-            else
+        uint4 wx[E], wy[E], wh[E], wd[E];
 #pragma unroll
-                for (int e = 0; e < K; ++e) d[e] = 0.f;
-            row.template gate<GV>(a, r, g);
+        for (int j = 0; j < E; ++j) wh[j] = wd[j] = make_uint4(0, 0, 0, 0);
+        auto ask = [&](int64_t r) {
+            row.ask(a.y, r * a.C, wy);
+            row.ask(a.x, r * a.C, wx);
+            if (a.d_h) row.ask(a.d_h, r * a.C, wh);
+            if (a.d_out) row.ask(a.d_out, r * a.C, wd);
+        };
+        int64_t r = group * a.span + first + threadIdx.x / LPR;
+        if (r < r1) ask(r);
+        for (; r < r1; r += ROWS) {
+            float z[K], t[K], d[K], u[K], zz[K];
+            row.take(wy, z);
+            row.take(wx, t);
+            row.take(wh, u);
+            row.take(wd, d);
+            if (r + ROWS < r1) ask(r + ROWS);
+            row.template gate<GV>(a, r, held, g);
             float zr = 0.f;
             if (a.post) {
                 zr = row.norm(z, a.rms, a.eps, rs);                // z holds zhat from here on
-                row.param(a, a.post_b, 0.f, b);
+                row.param(a, a.post_b, 0.f, zz);
+#pragma unroll
+                for (int e = 0; e < K; ++e) zz[e] = fmaf(z[e], pw[e], zz[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < K; ++e) zz[e] = z[e];
             }
             if (a.d_h) {
 #pragma unroll
-                for (int e = 0; e < K; ++e) t[e] = fmaf(sc[e] * a.scale_value * g[GV ? e : 0], a.post ? fmaf(z[e], pw[e], b[e]) : z[e], t[e]);
+                for (int e = 0; e < K; ++e) t[e] = fmaf(sc[e] * g[GV ? e : 0], zz[e], t[e]);
                 const float hr = row.norm(t, a.rms, a.eps, rs);
 #pragma unroll
                 for (int e = 0; e < K; ++e) {
@@ -297,13 +380,12 @@ __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_bwd_kernel(Rn
             float gs = 0.f;
 #pragma unroll
             for (int e = 0; e < K; ++e) {
-                const float zz = a.post ? fmaf(z[e], pw[e], b[e]) : z[e];
-                const float dz = d[e] * zz * a.scale_value;        // gradient of s_c a
+                const float dz = d[e] * zz[e];                     // gradient of the factor scale_value * scale * a
                 acc[P_SCALE][e] = fmaf(dz, g[GV ? e : 0], acc[P_SCALE][e]);
                 u[e] = dz * sc[e];                                 // gradient of a
                 if constexpr (GV) ga[e] += u[e];
                 else gs += u[e];
-                d[e] *= sc[e] * a.scale_value * g[GV ? e : 0];              // gradient of z
+                d[e] *= sc[e] * g[GV ? e : 0];                     // gradient of z
             }
             if (a.want & 256) {
                 if constexpr (GV) {
@@ -332,7 +414,7 @@ __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_bwd_kernel(Rn
         }
         if (a.want & 256) {
             if constexpr (GV) {
-                if (a.gate_mode == GATE_GROUP) block_columns(row, ga, a.gparts + item * a.C);
+                if (a.gate_mode == GATE_GROUP) block_columns(row, ga, 1.f, a.gparts + item * a.C);
             } else if (a.gate_mode == GATE_GROUP_ONE) {
                 const float s1 = wave_sum_nolds(ga[0]);
                 __syncthreads();
@@ -348,7 +430,7 @@ __global__ __launch_bounds__(rn_threads<LPR>()) void residual_norm_bwd_kernel(Rn
     }
 #pragma unroll
     for (int q = 0; q < NPARAM; ++q)
-        if (a.want >> q & 1) block_columns(row, acc[q], a.parts + ((int64_t)blockIdx.x * NPARAM + q) * a.C);
+        if (a.want >> q & 1) block_columns(row, acc[q], q == P_SCALE ? a.scale_value : 1.f, a.parts + ((int64_t)blockIdx.x * NPARAM + q) * a.C);
 }
 
 // the second launch: parameter columns over all blocks, gate groups over their chunks.  A block owns 16 columns; its 16 row lanes add the
@@ -406,43 +488,41 @@ __global__ __launch_bounds__(256) void residual_norm_reduce_kernel(RnReduce a) {
     }
 }
 
-// lanes of a row and vectors of a lane: 16 lanes while 8 elements each hold the row, then a wave, then 4, then 8 waves; 16-byte vectors where
-// the channel count and every address allow them.  (16 elements a lane take all 256 VGPRs of the backward kernel and 1 wave a SIMD.)
-struct RnShape { int lpr, e; bool vec; };
-RnShape rn_shape(int C, int n, bool vec) {
-    RnShape s{vec && C <= 128 ? 16 : (C <= 512 ? 64 : (C <= 2048 ? 256 : 512)), 8 / n, vec};
-    if (!vec) s.e = 8;
+// lanes of a row and 16-byte vectors of a lane: 16 lanes while 8 elements each hold the row, then a wave, then 4, then 8 waves.  (16 elements
+// a lane take all 256 VGPRs of the backward kernel and spill: above 4 096 channels only.)
+struct RnShape { int lpr, e; };
+RnShape rn_shape(int C, int n) {
+    RnShape s{C <= 128 ? 16 : (C <= 512 ? 64 : (C <= 2048 ? 256 : 512)), 8 / n};
     if (s.lpr == 512 && C > 4096) s.e *= 2;
-    if (vec && n == 4 && C <= s.lpr * 4) s.e = 1;
+    if (n == 4 && s.lpr < 512 && C <= s.lpr * 4) s.e = 1;
     return s;
 }
-template <typename T, int N, int LPR, int E>
-void rn_go(bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
+template <typename T, int LPR, int E, int FIT>
+void rn_fit(bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
     const dim3 b(rn_threads<LPR>());
-    if (!bwd) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, N, LPR, E>), dim3(grid), b, 0, st, a);
-    else if (a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, N, LPR, E, true>), dim3(grid), b, 0, st, a);
-    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, N, LPR, E, false>), dim3(grid), b, 0, st, a);
+    if (!bwd) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, LPR, E, FIT>), dim3(grid), b, 0, st, a);
+    else if (a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, LPR, E, FIT, true>), dim3(grid), b, 0, st, a);
+    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, LPR, E, FIT, false>), dim3(grid), b, 0, st, a);
 }
-template <typename T, int N, int LPR>
+template <typename T, int LPR, int E>
+void rn_go(bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
+    if (a.C == LPR * E * Vec16<T>::N) rn_fit<T, LPR, E, EXACT>(bwd, a, grid, st);
+    else rn_fit<T, LPR, E, ANY>(bwd, a, grid, st);
+}
+template <typename T, int LPR>
 void rn_e(int e, bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
-    constexpr int E = 8 / N;
-    if constexpr (N == 4 && LPR < 512) if (e == 1) return rn_go<T, N, LPR, 1>(bwd, a, grid, st);
-    if constexpr (LPR == 512) if (e == 2 * E) return rn_go<T, N, LPR, 2 * E>(bwd, a, grid, st);
-    rn_go<T, N, LPR, E>(bwd, a, grid, st);
+    constexpr int E = 8 / Vec16<T>::N;
+    if constexpr (E == 2 && LPR < 512) if (e == 1) return rn_go<T, LPR, 1>(bwd, a, grid, st);
+    if constexpr (LPR == 512) if (e == 2 * E) return rn_go<T, LPR, 2 * E>(bwd, a, grid, st);
+    rn_go<T, LPR, E>(bwd, a, grid, st);
 }
 template <typename T>
 int rn_launch(const RnShape &s, bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
-    constexpr int N = 16 / sizeof(T);
-    if (s.vec) {
-        if (s.lpr == 16) rn_e<T, N, 16>(s.e, bwd, a, grid, st);
-        else if (s.lpr == 64) rn_e<T, N, 64>(s.e, bwd, a, grid, st);
-        else if (s.lpr == 256) rn_e<T, N, 256>(s.e, bwd, a, grid, st);
-        else rn_e<T, N, 512>(s.e, bwd, a, grid, st);
-    } else {
-        if (s.lpr == 64) rn_e<T, 1, 64>(s.e, bwd, a, grid, st);
-        else if (s.lpr == 256) rn_e<T, 1, 256>(s.e, bwd, a, grid, st);
-        else rn_e<T, 1, 512>(s.e, bwd, a, grid, st);
-    }
+    if (a.C < Vec16<T>::N) rn_fit<T, 16, 1, TINY>(bwd, a, grid, st);
+    else if (s.lpr == 16) rn_e<T, 16>(s.e, bwd, a, grid, st);
+    else if (s.lpr == 64) rn_e<T, 64>(s.e, bwd, a, grid, st);
+    else if (s.lpr == 256) rn_e<T, 256>(s.e, bwd, a, grid, st);
+    else rn_e<T, 512>(s.e, bwd, a, grid, st);
     return nmrf_launch_status();
 }
 int rn_dispatch(int dtype, const RnShape &s, bool bwd, const RnArgs &a, unsigned grid, hipStream_t st) {
@@ -501,13 +581,11 @@ extern "C" int nmrf_residual_norm(const void *x, const void *y, int64_t T, int C
     if (rc != NMRF_OK) return rc;
     if (T == 0) return NMRF_OK;
     if (!x || !y || !out) return NMRF_ENULL;
-    const int n = dtype == NMRF_F32 ? 4 : 8;
-    const void *gv = a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP ? gate : nullptr;
-    const RnShape s = rn_shape(C, n, C % n == 0 && rn_aligned({x, y, gv, out, h}, 15));
-    a.pvec = rn_aligned({post_w, post_b, next_w, next_b, scale}, 15);
+    const RnShape s = rn_shape(C, dtype == NMRF_F32 ? 4 : 8);
     const int rows = s.lpr <= 256 ? 256 / s.lpr : 1;
-    int64_t grid = ceil_div64(T, rows);
-    if (grid > 2048) grid = 2048;
+    const int64_t most = s.lpr < 256 ? 2048 : (s.lpr == 256 ? 1024 : 512);
+    a.rows_per_item = ceil_div64(ceil_div64(T, most), rows) * rows;
+    const int64_t grid = ceil_div64(T, a.rows_per_item);
     return rn_dispatch(dtype, s, false, a, (unsigned)grid, (hipStream_t)stream);
 }
 
@@ -540,10 +618,7 @@ extern "C" int nmrf_residual_norm_bwd(const void *x, const void *y, const void *
     void *to[NPARAM] = {d_next_w, d_next_b, d_scale, d_post_w, d_post_b};
     for (int q = 0; q < NPARAM; ++q) a.want |= to[q] ? 1 << q : 0;
     if (dgate) a.want |= 256;
-    const int n = dtype == NMRF_F32 ? 4 : 8;
-    const bool gvec = a.gate_mode == GATE_ELEM || a.gate_mode == GATE_GROUP;
-    const RnShape s = rn_shape(C, n, C % n == 0 && rn_aligned({x, y, d_out, d_h, dx, dy, gvec ? gate : nullptr, a.gate_mode == GATE_ELEM ? dgate : nullptr}, 15));
-    a.pvec = rn_aligned({post_w, post_b, next_w, scale}, 15);
+    const RnShape s = rn_shape(C, dtype == NMRF_F32 ? 4 : 8);
     // rows are dealt out group by group only where a gate gradient is summed over them
     const bool grouped = dgate && (a.gate_mode == GATE_GROUP || a.gate_mode == GATE_GROUP_ONE);
     a.R = gate ? gate_rows : 1;
