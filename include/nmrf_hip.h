@@ -40,8 +40,8 @@ const char *nmrf_strerror(int code);
  * in a separate pass when range_flag != NULL; pass NULL when qkv was produced by nmrf_nmp_block16_f32, which range-checks its q_out. */
 int nmrf_range_scan_f32(const float *x, int64_t n, int *range_flag, void *stream);   /* n % 4 == 0, x 16-byte aligned */
 /* ABI version of this header; bumps on any signature change. */
-#define NMRF_ABI_VERSION 29
-#define NMRF_ABI_STR "29"
+#define NMRF_ABI_VERSION 30
+#define NMRF_ABI_STR "30"
 int nmrf_abi_version(void);   /* = NMRF_ABI_VERSION */
 /* "abi<version>-<16 hex digits>": the digits are a hash of every source and header the library was built from (python -m
  * nmrf_amd.build).  The tools library (libnmrf_hip_debug.so) of the same build returns the same string; the binding refuses one that
@@ -559,6 +559,24 @@ int nmrf_residual_norm_bwd(const void *x, const void *y, const void *d_out, cons
                            const void *scale, int post, const void *post_w, const void *post_b, const void *next_w, int params_f32,
                            void *dx, void *dy, void *dgate, void *d_scale, void *d_post_w, void *d_post_b, void *d_next_w,
                            void *d_next_b, float *ws, int64_t ws_floats, void *stream);
+
+/* The gated feed-forward block (csrc/gated_ffn.hip; the reference's own feed-forward is the ungated fc2(gelu(fc1 x)), nmrf/models/NMP.py:337,
+ * 537, 675):  h = act(x w_gate^T + b_gate) * (x w_up^T + b_up),  y = h w_down^T + b_down.
+ * x [T, D], w_gate, w_up [F, D], w_down [Do, F], biases [F], [F], [Do] (each may be NULL), all of type dtype; D, F, Do <= 2^22; act 0 silu,
+ * 1 gelu (erf), 2 relu.  -> h [T, F] (workspace of inference, operand of the backward pass), y [T, Do]; g, u [T, F]: the two projections,
+ * which the backward pass reads (both NULL: not kept; up to 64 rows then stream the weights once).  amax [384]: largest magnitudes of fp32
+ * operands (workspace of inference; the backward pass takes it; unused and may be NULL for 16-bit types).  Outputs may not overlap inputs. */
+int nmrf_gated_ffn(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *b_gate, const void *b_up,
+                   const void *b_down, int64_t T, int D, int F, int Do, int dtype, int act, void *h, void *g, void *u, void *y,
+                   uint32_t *amax, void *stream);
+/* floats of the workspace of nmrf_gated_ffn_bwd (partial weight gradients); its reference is autograd (main.py:413-430). */
+int nmrf_gated_ffn_bwd_size(int64_t T, int D, int F, int Do, int dtype, int64_t *floats);
+/* Its backward pass (reference: autograd of the blocks, main.py:413-430) from h, g, u and amax of the forward pass and dy [T, Do]: dg, du [T, F]
+ * (workspace), dx [T, D], dw_* and db_* in the shapes of w_* and b_* (each may be NULL: not asked for).  amax is updated.  T >= 1. */
+int nmrf_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *g, const void *u,
+                       const void *dy, int64_t T, int D, int F, int Do, int dtype, int act, void *dg, void *du, void *dx, void *dw_gate,
+                       void *dw_up, void *dw_down, void *db_gate, void *db_up, void *db_down, uint32_t *amax, float *ws,
+                       int64_t ws_floats, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1566,3 +1566,36 @@ def residual_norm_backward(x, y, gate, scale, post_w, post_b, next_w, next_b, d_
                                                   _p(next_w), s.params_f32, _p(dx), _p(dy), dg, dsc, dpw, dpb, dnw, dnb, _p(ws), ws.numel(),
                                                   _raw_stream()), "residual_norm_bwd")
     return [dx, dy] + grads
+
+
+@_on_device
+def gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
+    """x [T, D] -> (y, h, g, u, amax); g, u None without `keep` (the backward pass needs them), amax None for 16-bit types."""
+    t, d = x.shape
+    f, do = w_gate.shape[0], w_down.shape[0]
+    y, h = x.new_empty(t, do), x.new_empty(t, f)
+    g, u = (x.new_empty(t, f), x.new_empty(t, f)) if keep else (None, None)
+    amax = torch.empty(384, device=x.device, dtype=torch.int32) if x.dtype == torch.float32 else None
+    _lib.check(_lib.load().nmrf_gated_ffn(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(b_gate), _p(b_up), _p(b_down), t, d, f, do, DTYPE_CODE[x.dtype],
+                                          act, _p(h), _p(g), _p(u), _p(y), _p(amax), _raw_stream()), "gated_ffn")
+    return y, h, g, u, amax
+
+
+@_on_device
+def gated_ffn_backward(x, w_gate, w_up, w_down, h, g, u, amax, dy, act, want):
+    """-> gradients of (x, w_gate, w_up, w_down, b_gate, b_up, b_down); want: which of them (None elsewhere)."""
+    t, d = x.shape
+    f, do = w_gate.shape[0], w_down.shape[0]
+    shapes = ((t, d), (f, d), (f, d), (do, f), (f,), (f,), (do,))
+    if t == 0:
+        return [x.new_zeros(s) if w else None for s, w in zip(shapes, want)]
+    grads = [x.new_empty(s) if w else None for s, w in zip(shapes, want)]
+    dg, du = torch.empty_like(g), torch.empty_like(u)
+    size = ctypes.c_int64()
+    lib = _lib.load()
+    _lib.check(lib.nmrf_gated_ffn_bwd_size(t, d, f, do, DTYPE_CODE[x.dtype], ctypes.byref(size)), "gated_ffn_bwd")
+    ws = torch.empty(size.value, device=x.device, dtype=torch.float32)
+    amax = None if amax is None else amax.clone()                      # (a second backward pass of one graph may run beside this one)
+    _lib.check(lib.nmrf_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(h), _p(g), _p(u), _p(dy), t, d, f, do, DTYPE_CODE[x.dtype], act,
+                                      _p(dg), _p(du), *[_p(v) for v in grads], _p(amax), _p(ws), ws.numel(), _raw_stream()), "gated_ffn_bwd")
+    return grads

@@ -1,6 +1,7 @@
-"""Operators of a training block as autograd Functions over the HIP kernels: the norms around it with its gate and residual scale
-(csrc/residual_norm.hip).  They stand beside the reference's block tails, x + proj(attn) / x + mlp(norm2(x)) (nmrf/models/NMP.py:337-364),
-their post-norm form (NMP.py:366-382) and stochastic depth (nmrf/models/swin.py:228-233, 300-301)."""
+"""Operators of a training block as autograd Functions over the HIP kernels: the gated feed-forward block (csrc/gated_ffn.hip) and the norms
+around a block with its gate and residual scale (csrc/residual_norm.hip).  They stand beside the reference's feed-forward, fc2(gelu(fc1 x))
+(nmrf/models/NMP.py:337, 537, 675), its block tails, x + proj(attn) / x + mlp(norm2(x)) (NMP.py:337-364), their post-norm form
+(NMP.py:366-382) and stochastic depth (nmrf/models/swin.py:228-233, 300-301)."""
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -117,3 +118,52 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
     x, y = x.contiguous(), y.contiguous()
     gate = None if gate is None else gate.contiguous()
     return ResidualNormFn.apply(x, y, gate, vec, post_w, post_b, next_w, next_b, s)
+
+
+_FFN_ACTS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+class GatedFfnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
+        keep = any(ctx.needs_input_grad)
+        y, h, g, u, amax = K.gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep)
+        if keep:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, h, g, u, amax)
+            ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        refuse_captured_backward("gated_ffn")
+        return (*K.gated_ffn_backward(*ctx.saved_tensors, dy.contiguous(), ctx.act, ctx.needs_input_grad[:7]), None)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu"):
+    """y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: both projections, the activation and the product in one kernel, the
+    second matrix in another.
+
+    x: [..., D]; w_gate, w_up: [F, D]; w_down: [D', F]; biases [F], [F], [D'], each may be None; one type, fp32 / bf16 / fp16 (copied where not
+    contiguous).  act: "silu", "gelu" (erf) or "relu".  16-bit types multiply on the matrix pipe as they are (sums in fp32; h and, for the
+    backward pass, both projections are kept in the type); fp32 is multiplied as scaled fp16 pairs: errors of 2^-22 relative to each operand's
+    largest entry, and an infinite input gives NaN.  Differentiable in every tensor, the same bits every run.  Up to 64 rows without gradients
+    (decoding) stream the weights once.  The forward pass may be captured into a graph, the backward pass may not (it raises)."""
+    if act not in _FFN_ACTS:
+        raise ValueError("gated_ffn: act is 'silu', 'gelu' or 'relu', got %r" % (act,))
+    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2:
+        raise ValueError("gated_ffn: x [..., D], w_gate, w_up [F, D], w_down [D', F]; got %s, %s, %s" % (
+            tuple(x.shape), tuple(w_gate.shape), tuple(w_down.shape)))
+    d, (f, do) = x.shape[-1], (w_gate.shape[0], w_down.shape[0])
+    for name, t, shape in (("w_gate", w_gate, (f, d)), ("w_up", w_up, (f, d)), ("w_down", w_down, (do, f)), ("b_gate", b_gate, (f,)),
+                           ("b_up", b_up, (f,)), ("b_down", b_down, (do,))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError("gated_ffn: %s has shape %s, expected %s" % (name, tuple(t.shape), shape))
+    if min(d, f, do) < 1 or max(d, f, do) > 1 << 22:
+        raise ValueError("gated_ffn: widths %d, %d, %d are not in 1 ... 2^22" % (d, f, do))
+    check_rows("gated_ffn", x=x, w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down)
+    rows = x.numel() // d
+    if rows > 0x7fffffff - 256:
+        raise ValueError("gated_ffn: %d rows" % rows)
+    args = [None if t is None else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    return GatedFfnFn.apply(x.reshape(rows, d).contiguous(), *args, _FFN_ACTS[act]).view(*x.shape[:-1], do)
