@@ -563,17 +563,18 @@ int nmrf_residual_norm_bwd(const void *x, const void *y, const void *d_out, cons
 /* The gated feed-forward block (csrc/gated_ffn.hip; the reference's own feed-forward is the ungated fc2(gelu(fc1 x)), nmrf/models/NMP.py:337,
  * 537, 675):  h = act(x w_gate^T + b_gate) * (x w_up^T + b_up),  y = h w_down^T + b_down.
  * x [T, D], w_gate, w_up [F, D], w_down [Do, F], biases [F], [F], [Do] (each may be NULL), all of type dtype; D, F, Do <= 2^22; act 0 silu,
- * 1 gelu (erf), 2 relu.  -> h [T, F] (workspace of inference, operand of the backward pass), y [T, Do]; g, u [T, F]: the two projections,
- * which the backward pass reads (both NULL: not kept; up to 64 rows then stream the weights once).  amax [384]: largest magnitudes of fp32
- * operands (workspace of inference; the backward pass takes it; unused and may be NULL for 16-bit types).  Outputs may not overlap inputs. */
+ * 1 gelu (erf), 2 relu.  -> h [T, F] (workspace of inference, operand of the backward pass), y [T, Do]; g, u [T, F] in fp32: the two
+ * projections, which the backward pass reads (both NULL: not kept; up to 64 rows then stream the weights once).  amax [1792]: largest
+ * magnitudes of fp32 operands (workspace of inference; the backward pass takes it; unused and may be NULL for 16-bit types).  ws: fp32
+ * workspace of nmrf_gated_ffn_size floats (may be NULL for 0, and for up to 64 rows without g, u).  Outputs may not overlap inputs. */
 int nmrf_gated_ffn(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *b_gate, const void *b_up,
-                   const void *b_down, int64_t T, int D, int F, int Do, int dtype, int act, void *h, void *g, void *u, void *y,
-                   uint32_t *amax, void *stream);
-/* floats of the workspace of nmrf_gated_ffn_bwd (partial weight gradients); its reference is autograd (main.py:413-430). */
-int nmrf_gated_ffn_bwd_size(int64_t T, int D, int F, int Do, int dtype, int64_t *floats);
+                   const void *b_down, int64_t T, int D, int F, int Do, int dtype, int act, void *h, float *g, float *u, void *y,
+                   uint32_t *amax, float *ws, int64_t ws_floats, void *stream);
+/* floats of the workspace of nmrf_gated_ffn (backward == 0) and nmrf_gated_ffn_bwd: partial products; its reference is autograd (main.py:413-430). */
+int nmrf_gated_ffn_size(int64_t T, int D, int F, int Do, int dtype, int backward, int64_t *floats);
 /* Its backward pass (reference: autograd of the blocks, main.py:413-430) from h, g, u and amax of the forward pass and dy [T, Do]: dg, du [T, F]
  * (workspace), dx [T, D], dw_* and db_* in the shapes of w_* and b_* (each may be NULL: not asked for).  amax is updated.  T >= 1. */
-int nmrf_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *g, const void *u,
+int nmrf_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const float *g, const float *u,
                        const void *dy, int64_t T, int D, int F, int Do, int dtype, int act, void *dg, void *du, void *dx, void *dw_gate,
                        void *dw_up, void *dw_down, void *db_gate, void *db_up, void *db_down, uint32_t *amax, float *ws,
                        int64_t ws_floats, void *stream);

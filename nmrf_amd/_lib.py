@@ -94,8 +94,8 @@ PROTOTYPES = {
     "nmrf_adamw_moment_f32": [_P, _P, _L, _I, _P, _P],
     "nmrf_grad_sqsum": [_I, _P, _P, _I, _P, _L, _P],
     "nmrf_grad_norm": [_P, _L, _F, _P, _P],
-    "nmrf_gated_ffn": [_P] * 7 + [_L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P],
-    "nmrf_gated_ffn_bwd_size": [_L, _I, _I, _I, _I, _P],
+    "nmrf_gated_ffn": [_P] * 7 + [_L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _L, _P],
+    "nmrf_gated_ffn_size": [_L, _I, _I, _I, _I, _I, _P],
     "nmrf_gated_ffn_bwd": [_P] * 8 + [_L, _I, _I, _I, _I, _I] + [_P] * 10 + [_P, _L, _P],
     "nmrf_residual_norm": [_P, _P, _L, _I, _I, _I, _F, _P, _L, _I, _I, _F, _P, _I, _P, _P, _P, _P, _I, _P, _P, _P],
     "nmrf_residual_norm_bwd_size": [_L, _I, _L, _P],

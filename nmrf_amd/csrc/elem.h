@@ -81,6 +81,18 @@ template <typename T> struct Vec16 {
             }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // the first n <= N values, zeros behind them, where `room` values from p on may be read
+    static __device__ __forceinline__ uint4 raw_masked(const T *p, int n, int64_t room) {
+        if (room < N) return raw_part(p, n < room ? n : (int)room);
+        const uint4 t = raw(p);
+        unsigned w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) w[j] = j < n ? w[j] : 0u;
+            else w[j] &= (2 * j < n ? 0xffffu : 0u) | (2 * j + 1 < n ? 0xffff0000u : 0u);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     static __device__ __forceinline__ void store_part(T *p, const float *v, int n) {
 #pragma unroll
         for (int k = 0; k < N; ++k)

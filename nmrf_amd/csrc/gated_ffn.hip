@@ -15,6 +15,7 @@
 // operand layout without LDS, a block's 8 waves sharing the contraction.
 #include "common.h"
 #include "elem.h"
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -33,54 +34,68 @@ __device__ __forceinline__ f32x4 mma(const uint4 &a, const uint4 &b, f32x4 c, __
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
+// act(g) and its derivative.  gelu: Phi(g) from erfc(|g| / sqrt 2) = 2^(-t P(t)), t = min(|g|, 7), the polynomial of gelu_fast (common.h: off by
+// 5.3e-8 in Phi's scale), one more exponential for the density in the derivative.
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
-__device__ __forceinline__ float act_value(float g, int act) {
-    if (act == ACT_SILU) return g / (1.0f + expf(-g));
-    if (act == ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f));
-    return g > 0.f ? g : (g != g ? g : 0.f);
-}
-__device__ __forceinline__ float act_slope(float g, int act) {
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ __forceinline__ void act_both(float g, int act, float &value, float &slope) {
     if (act == ACT_SILU) {
-        const float s = 1.0f / (1.0f + expf(-g));
-        return s * (1.0f + g * (1.0f - s));
+        const float s = 1.0f / (1.0f + exp_of(-g));
+        value = g == -INFINITY ? 0.f : g * s;
+        slope = fmaf(value, 1.0f - s, s);
+    } else if (act == ACT_GELU) {
+        const float t = fminf(fabsf(g), 7.0f);
+        float p = fmaf(-3.0177725420799106e-05f, t, 0.0007414184510707855f);
+        p = fmaf(p, t, -0.007980725727975368f);
+        p = fmaf(p, t, 0.053240980952978134f);
+        p = fmaf(p, t, 0.45891475677490234f);
+        p = fmaf(p, t, 1.151147484779358f);
+        const float half = 0.5f * __builtin_amdgcn_exp2f(-t * p), phi = g < 0.f ? half : 1.0f - half;
+        value = g == -INFINITY ? 0.f : g * phi;
+        slope = fmaf(t * (g < 0.f ? -0.39894228040143267794f : 0.39894228040143267794f), exp_of(-0.5f * t * t), phi);
+        if (g != g) value = slope = g;
+    } else {
+        value = g > 0.f ? g : (g != g ? g : 0.f);
+        slope = g > 0.f ? 1.f : 0.f;
     }
-    if (act == ACT_GELU) return 0.5f * (1.0f + erff(g * 0.70710678118654752440f)) + g * 0.39894228040143267794f * expf(-0.5f * g * g);
-    return g > 0.f ? 1.f : 0.f;
+}
+__device__ __forceinline__ float act_value(float g, int act) {
+    float v, s;
+    act_both(g, act, v, s);
+    return v;
 }
 
-// ---- largest magnitudes (fp32 operands): per tensor 64 slots, of which a product takes the maximum --------------------------------------
-enum { SLOT_X = 0, SLOT_W = 1, SLOT_WD = 2, SLOT_H = 3, SLOT_DY = 4, SLOT_DG = 5, NSLOT = 6 };
-struct AbsmaxArgs { const float *p[5]; int64_t n[5]; int slot[5]; int count; unsigned *out; int zero; };      // zero: bit i clears slot i
+// ---- largest magnitudes (fp32 operands): per tensor 256 slots, of which a product takes the maximum --------------------------------------
+enum { SLOT_X = 0, SLOT_WG = 1, SLOT_WU = 2, SLOT_WD = 3, SLOT_H = 4, SLOT_DY = 5, SLOT_DG = 6 };
+struct AbsmaxArgs { const float *p[5]; int64_t n[5]; int slot[5]; unsigned *out; };      // p null: clear the slot (a later kernel fills it)
 __global__ __launch_bounds__(256) void ffn_absmax_kernel(AbsmaxArgs a) {
     __shared__ float sh[4];
     const int which = blockIdx.y;
     const float *p = a.p[which];
-    const int64_t n = a.n[which], per = (n + gridDim.x - 1) / gridDim.x, i0 = blockIdx.x * per, i1 = min(n, i0 + per);
+    const int64_t n = p ? a.n[which] : 0, per = (n + 1023) / 1024 * 4, i0 = blockIdx.x * per, i1 = min(n, i0 + per);
     float m[4] = {0.f, 0.f, 0.f, 0.f};
     int64_t i = i0 + threadIdx.x * 4;
-    for (; i + 4 <= i1; i += 1024) {
-        float v[4];
-        Vec16<float>::unpack(Vec16<float>::raw(p + i), v);
+    for (; i + 3076 <= i1; i += 4096) {                            // four loads in flight
+        float v[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], fabsf(v[k]));
+        for (int u = 0; u < 4; ++u) Vec16<float>::unpack(Vec16<float>::raw(p + i + 1024 * u), v[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], fabsf(v[u][k]));
     }
-    for (; i < i1; ++i) m[0] = fmaxf(m[0], fabsf(p[i]));          // (a lane's last quad, cut short)
+    for (; i < i1; i += 1024)
+        for (int k = 0; k < 4 && i + k < i1; ++k) m[k] = fmaxf(m[k], fabsf(p[i + k]));
     float x = wave_max(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        x = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-        unsigned *o = a.out + a.slot[which] * 64 + (blockIdx.x & 63);     // (cleared by the launch before; the maximum does not depend on the order)
-        atomicMax(o, __float_as_uint(x));
-    }
-}
-__global__ void ffn_zero_kernel(unsigned *out, int zero) {
-    if (zero >> blockIdx.x & 1) out[blockIdx.x * 64 + threadIdx.x] = 0u;
+    if (threadIdx.x == 0) a.out[a.slot[which] * 256 + blockIdx.x] = __float_as_uint(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
 }
 // power of two that puts the largest magnitude at [2^13, 2^14); 1 for zero, infinity and NaN
-__device__ __forceinline__ int slot_shift(const unsigned *amax, int slot) {
-    if (!amax) return 0;
-    float m = wave_max(__uint_as_float(amax[slot * 64 + (threadIdx.x & 63)]));
+__device__ __forceinline__ int slot_shift(const unsigned *amax, int slot, int count) {
+    float m = 0.f;
+    for (int i = threadIdx.x & 63; i < 256 * count; i += 64) m = fmaxf(m, __uint_as_float(amax[slot * 256 + i]));
+    m = wave_max(m);
     if (!(m > 0.f) || !(m < INFINITY)) return 0;
     const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127, sh = 13 - (e < -100 ? -100 : e);
     return __builtin_amdgcn_readfirstlane(sh);
@@ -94,8 +109,8 @@ struct GemmArgs {
     const void *P[2], *Q[2];
     int64_t ldp, ldq, ldc;
     int M, N, K, segs;                           // K of one segment
-    void *C, *C2, *C3;                           // EPI_DUAL: h, g, u (C2, C3 may be null); EPI_PLAIN: the product; EPI_DH: dg, du in C, C2
-    const void *g, *u;                           // EPI_DH
+    void *C, *C2, *C3;                           // EPI_DUAL: h, g, u (C2, C3 fp32, may be null); EPI_PLAIN: the product; EPI_DH: dg, du in C, C2
+    const float *g, *u;                          // EPI_DH
     const void *bias, *bias2;
     float *parts;                                // EPI_PLAIN with splits > 1: fp32 partial products [splits][M][N]
     unsigned *amax;                              // fp32: the slots above
@@ -117,32 +132,22 @@ template <typename T, int ROWS, int BK, bool ALONG, int THREADS> struct Stage {
         if constexpr (ALONG) return c ^ ((i / (16 / CPR)) & (CPR - 1));
         else return c ^ ((2 * ((i & 3) | ((i >> 3) & 1) << 2)) & (CPR - 1));
     }
-    // base: the operand's element (m0, k0) (block and k tile), rows: valid rows m, kleft: valid k.  row(m): offset of row m from base.
+    // The operand's tile (rows from m0, contraction from k0).  row_of(i, end): address of (row i of the tile, k0) and of the tensor's end, for
+    // ALONG; base: address of (k0, m0), for ACROSS.  left: values of k from k0 on; rows: rows from m0 on.  A row behind the last is read as
+    // another one (its products are not stored), a value of k behind the last is zero.
     template <typename RowOf>
-    __device__ __forceinline__ void load(const T *base, int64_t ld, int rows, int kleft, bool whole, RowOf row_of) {
+    __device__ __forceinline__ void load(const T *base, int ld, int rows, int left, const T *end, RowOf row_of) {
+        // ACROSS reads over a row's end into the rows behind it (8 of them hold 8 values whatever their width) unless the rows end with a chunk
+        const bool whole = left >= (ALONG || (rows & 7) == 0 ? BK : BK + 8);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int id = threadIdx.x + n * THREADS, i = id / CPR, c = id % CPR;
-            if constexpr (ALONG) {
-                const T *p = row_of(i) + c * 8;
-                if (whole) {
+            const int id = threadIdx.x + n * THREADS, i = id / CPR, c = id % CPR * 8;
+            const T *p = ALONG ? row_of(i, end) + c : base + (unsigned)((whole || i < left ? i : 0) * ld) + (c < rows ? c : 0);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) r[n][v] = Vec16<T>::raw(p + v * (8 / V));
-                } else {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) r[n][v] = Vec16<T>::raw_part(p + v * (8 / V), max(0, min(8 / V, kleft - c * 8 - v * (8 / V))));
-                }
-            } else {
-                if (whole) {
-                    const T *p = base + (int64_t)(unsigned)(i * (int)ld) + (c * 8 < rows ? c * 8 : 0);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) r[n][v] = Vec16<T>::raw(p + v * (8 / V));
-                } else {
-                    const int left = i < kleft ? rows - c * 8 : 0;
-                    const T *p = base + (int64_t)(i < kleft ? i : 0) * ld + (left > 0 ? c * 8 : 0);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) r[n][v] = Vec16<T>::raw_part(p + v * (8 / V), max(0, min(8 / V, left - v * (8 / V))));
-                }
+            for (int v = 0; v < V; ++v) {
+                const T *q = p + v * (8 / V);
+                if (whole) r[n][v] = Vec16<T>::raw(q);
+                else r[n][v] = Vec16<T>::raw_masked(q, ALONG ? max(0, left - c - v * (8 / V)) : (i < left ? 8 : 0), end - q);
             }
         }
     }
@@ -216,7 +221,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     float pmul = 1.f, qmul = 1.f;
     int unshift = 0;
     if constexpr (PL == 2) {
-        const int sp_ = slot_shift(a.amax, a.slot_p), sq_ = slot_shift(a.amax, a.slot_q);
+        const int sp_ = slot_shift(a.amax, a.slot_p, 1), sq_ = slot_shift(a.amax, a.slot_q, a.slot_q == SLOT_WG ? 2 : 1);
         pmul = ldexpf(1.f, sp_);
         qmul = ldexpf(1.f, sq_);
         unshift = -(sp_ + sq_);
@@ -232,31 +237,31 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     SP sP;
     SQ sQ;
     auto fetch = [&](int kt) {
-        const int seg = kt / ktiles_seg, k0 = (kt - seg * ktiles_seg) * BK, kleft = a.K - k0;
-        const T *P = static_cast<const T *>(a.z > 1 ? (zz ? a.P[1] : a.P[0]) : (seg ? a.P[1] : a.P[0]));
+        const int seg = kt / ktiles_seg, k0 = (kt - seg * ktiles_seg) * BK, left = a.K - k0;
+        const T *P = static_cast<const T *>((a.z > 1 ? zz : seg) ? a.P[1] : a.P[0]);
         const T *Q = static_cast<const T *>(EPI != EPI_DUAL && seg ? a.Q[1] : a.Q[0]);
-        const bool kw = kleft >= BK;
-        // (a row behind the last is read as the last: its products are not stored)
+        auto none = [](int, const T *&) { return (const T *)nullptr; };
         if constexpr (PA) {
-            const T *b = P + (int64_t)m0 * a.ldp + k0;
-            sP.load(nullptr, 0, 0, kleft, kw, [&](int i) { return b + (unsigned)(min(i, prow - 1) * (int)a.ldp); });
+            const T *b = P + (int64_t)m0 * a.ldp + k0, *e = P + (int64_t)a.M * a.ldp;
+            sP.load(nullptr, 0, 0, left, e, [&](int i, const T *&) { return b + (unsigned)(min(i, prow - 1) * (int)a.ldp); });
         } else {
-            sP.load(P + (int64_t)k0 * a.ldp + m0, a.ldp, prow, kleft, kw && (prow >= BM || (a.M & 7) == 0), [](int) { return (const T *)nullptr; });
+            sP.load(P + (int64_t)k0 * a.ldp + m0, (int)a.ldp, prow, left, P + (int64_t)a.K * a.ldp, none);
         }
         if constexpr (QA) {
+            const T *b = Q + (int64_t)n0 * a.ldq + k0, *e = Q + (int64_t)a.N * a.ldq;
             if constexpr (EPI == EPI_DUAL) {
                 // of a wave's 16-column tiles the first half are Wg's rows, the second half Wu's
-                const T *b0 = Q + (int64_t)n0 * a.ldq + k0, *b1 = static_cast<const T *>(a.Q[1]) + (int64_t)n0 * a.ldq + k0;
-                sQ.load(nullptr, 0, 0, kleft, kw, [&](int i) {
+                const T *b1 = static_cast<const T *>(a.Q[1]) + (int64_t)n0 * a.ldq + k0, *e1 = static_cast<const T *>(a.Q[1]) + (int64_t)a.N * a.ldq;
+                sQ.load(nullptr, 0, 0, left, e, [&](int i, const T *&end) {
                     const int w = i / (TN * 16), j = i / 16 % TN, n = w * (TN * 8) + j % (TN / 2) * 16 + i % 16;
-                    return (j < TN / 2 ? b0 : b1) + (unsigned)(min(n, qrow - 1) * (int)a.ldq);
+                    end = j < TN / 2 ? e : e1;
+                    return (j < TN / 2 ? b : b1) + (unsigned)(min(n, qrow - 1) * (int)a.ldq);
                 });
             } else {
-                const T *b = Q + (int64_t)n0 * a.ldq + k0;
-                sQ.load(nullptr, 0, 0, kleft, kw, [&](int i) { return b + (unsigned)(min(i, qrow - 1) * (int)a.ldq); });
+                sQ.load(nullptr, 0, 0, left, e, [&](int i, const T *&) { return b + (unsigned)(min(i, qrow - 1) * (int)a.ldq); });
             }
         } else {
-            sQ.load(Q + (int64_t)k0 * a.ldq + n0, a.ldq, qrow, kleft, kw && (qrow >= BN || (a.N & 7) == 0), [](int) { return (const T *)nullptr; });
+            sQ.load(Q + (int64_t)k0 * a.ldq + n0, (int)a.ldq, qrow, left, Q + (int64_t)a.K * a.ldq, none);
         }
     };
     if (kt0 < kt1) {
@@ -318,6 +323,14 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
             for (int k = 0; k < left; ++k) p[k] = (T)v[k];
         }
     };
+    auto putf = [&](float *p, int left, const float *v) {
+        if (left >= 4) Vec16<float>::store(p, v);
+        else for (int k = 0; k < left; ++k) p[k] = v[k];
+    };
+    auto getf = [&](const float *p, int left, float *v) {
+        if (left >= 4) Vec16<float>::unpack(Vec16<float>::raw(p), v);
+        else for (int k = 0; k < 4; ++k) v[k] = k < left ? p[k] : 0.f;
+    };
     auto get4 = [&](const void *base, int64_t at, int left, float *v) {
         const T *p = static_cast<const T *>(base) + at;
         if (left >= 4) {
@@ -356,9 +369,9 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] += b[k];
                 }
-                if (a.C2) {
-                    put4(a.C2, at, left, v);
-                    put4(a.C3, at, left, w);
+                if (a.C2) {                                        // (kept in fp32: rounded to 16 bits they would double the gradients' error)
+                    putf(static_cast<float *>(a.C2) + at, left, v);
+                    putf(static_cast<float *>(a.C3) + at, left, w);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -368,21 +381,21 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
                 put4(a.C, at, left, v);
             } else if constexpr (EPI == EPI_DH) {
                 float g[4], u[4];
-                get4(a.g, at, left, g);
-                get4(a.u, at, left, u);
+                getf(static_cast<const float *>(a.g) + at, left, g);
+                getf(static_cast<const float *>(a.u) + at, left, u);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    w[k] = v[k] * act_value(g[k], a.act);
-                    v[k] = v[k] * u[k] * act_slope(g[k], a.act);
+                    float value, slope;
+                    act_both(g[k], a.act, value, slope);
+                    w[k] = v[k] * value;
+                    v[k] = v[k] * u[k] * slope;
                     if (k < left) top = fmaxf(top, fmaxf(fabsf(v[k]), fabsf(w[k])));
                 }
                 put4(a.C, at, left, v);
                 put4(a.C2, at, left, w);
             } else {
                 if (a.parts) {
-                    float *p = a.parts + ((int64_t)(zz * a.splits + sp) * a.M + m) * a.N + n;
-                    if (left >= 4) Vec16<float>::store(p, v);
-                    else for (int k = 0; k < left; ++k) p[k] = v[k];
+                    putf(a.parts + ((int64_t)(zz * a.splits + sp) * a.M + m) * a.N + n, left, v);
                 } else {
                     if (a.bias) {
                         float b[4];
@@ -398,50 +411,96 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     if constexpr (PL == 2 && EPI != EPI_PLAIN) {
         if (a.slot_out >= 0) {
             top = wave_max(top);
-            if (lane == 0) atomicMax(a.amax + a.slot_out * 64 + (blockIdx.x & 63), __float_as_uint(top));
+            if (lane == 0) atomicMax(a.amax + a.slot_out * 256 + (blockIdx.x & 255), __float_as_uint(top));
         }
     }
 }
 
-// partial products -> the product, in ascending order of the splits; z outputs
+// partial products [z][splits][n] -> the products (plus a bias of `cols` values): a block owns 256 values; its 4 row lanes add the splits l, l + 4,
+// ... in ascending order and the lane sums in ascending order
+struct JoinArgs { const float *parts[3]; void *c[3]; const void *bias; int64_t n[3]; int splits, cols; };
 template <typename T>
-__global__ __launch_bounds__(256) void ffn_join_kernel(const float *__restrict__ parts, int splits, int64_t n, T *c0, T *c1) {
-    const float *p = parts + (int64_t)blockIdx.y * splits * n;
-    T *c = blockIdx.y ? c1 : c0;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+__global__ __launch_bounds__(256) void ffn_join_kernel(JoinArgs a) {
+    __shared__ float sh[4][256];
+    const int64_t n = a.n[blockIdx.y];
+    const float *p = a.parts[blockIdx.y];
+    T *c = static_cast<T *>(a.c[blockIdx.y]);
+    const int l = threadIdx.x >> 6;
+    for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n; i0 += (int64_t)gridDim.x * 256) {
+        const int64_t i = i0 + (threadIdx.x & 63) * 4;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
-        const bool whole = i + 4 <= n;
-        for (int k = 0; k < splits; ++k) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            const float *q = p + (int64_t)k * n + i;
-            if (whole) Vec16<float>::unpack(Vec16<float>::raw(q), v);
-            else for (int e = 0; e < 4 && i + e < n; ++e) v[e] = q[e];
+        if (i + 4 <= n) {
+            int k = l;
+            for (; k + 12 < a.splits; k += 16) {                   // four loads in flight
+                float v[4][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += v[e];
+                for (int q = 0; q < 4; ++q) Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)(k + 4 * q) * n + i), v[q]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
+            }
+            for (; k < a.splits; k += 4) {
+                float v[4];
+                Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)k * n + i), v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += v[e];
+            }
+        } else {
+            for (int k = l; k < a.splits; k += 4)
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < n) s[e] += p[(int64_t)k * n + i + e];
         }
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (i + e < n) c[i + e] = (T)s[e];
+        for (int e = 0; e < 4; ++e) sh[l][(threadIdx.x & 63) * 4 + e] = s[e];
+        __syncthreads();
+        const int64_t j = i0 + threadIdx.x;
+        if (j < n) {
+            float v = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
+            if (a.bias) v += (float)static_cast<const T *>(a.bias)[j % a.cols];
+            c[j] = (T)v;
+        }
     }
 }
 
-// column sums (bias gradients): a block adds its rows of 64 columns (4 row lanes), the second launch adds the blocks' partials
+// column sums (bias gradients) of up to three matrices of T rows: a block adds its rows of 64 columns (16 row lanes of 16 column lanes), a join
+// adds the blocks' partials
+struct ColsumArgs { const void *x[3]; float *parts[3]; int cols[3]; int64_t rows, per; };
 template <typename T>
-__global__ __launch_bounds__(256) void ffn_colsum_kernel(const T *__restrict__ x, int64_t T_, int N, int64_t rows, float *__restrict__ parts) {
-    __shared__ float sh[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), l = threadIdx.x >> 6;
-    const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = min(T_, r0 + rows);
+__global__ __launch_bounds__(256) void ffn_colsum_kernel(ColsumArgs a) {
+    __shared__ float sh[16][65];
+    const int N = a.cols[blockIdx.z], c = blockIdx.x * 64 + (threadIdx.x & 15) * 4, l = threadIdx.x >> 4;
+    if (blockIdx.x * 64 >= N) return;
+    const T *x = static_cast<const T *>(a.x[blockIdx.z]);
+    const int64_t r0 = blockIdx.y * a.per, r1 = min(a.rows, r0 + a.per);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < N) {
+    if (c + 4 <= N) {
         int64_t r = r0 + l;
-        for (; r + 12 < r1; r += 16)
+        for (; r + 48 < r1; r += 64) {                             // four loads in flight
+            T v[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] += (float)x[(r + 4 * k) * N + c];
-        for (; r < r1; r += 4) s[0] += (float)x[r * N + c];
+            for (int k = 0; k < 4; ++k) __builtin_memcpy(v[k], x + (r + 16 * k) * N + c, 4 * sizeof(T));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += ((float)v[0][e] + (float)v[1][e]) + ((float)v[2][e] + (float)v[3][e]);
+        }
+        for (; r < r1; r += 16) {
+            T v[4];
+            __builtin_memcpy(v, x + r * N + c, 4 * sizeof(T));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += (float)v[e];
+        }
+    } else {
+        for (int64_t r = r0 + l; r < r1; r += 16)
+            for (int e = 0; e < 4 && c + e < N; ++e) s[e] += (float)x[r * N + c + e];
     }
-    sh[l][threadIdx.x & 63] = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[l][(threadIdx.x & 15) * 4 + e] = s[e];
     __syncthreads();
-    if (l == 0 && c < N) parts[(int64_t)blockIdx.y * N + c] = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
+    if (threadIdx.x < 64 && blockIdx.x * 64 + (int)threadIdx.x < N) {
+        float v = sh[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) v += sh[k][threadIdx.x];
+        a.parts[blockIdx.z][(int64_t)blockIdx.y * N + blockIdx.x * 64 + threadIdx.x] = v;
+    }
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------------------------
@@ -543,15 +602,52 @@ void few_launch(const FewArgs &a, hipStream_t st) {
     else hipLaunchKernelGGL((ffn_few_kernel<T, NW, 4>), g, b, 0, st, a);
 }
 
+// Tiles of 128 x 128 where they fill the chip, of 64 x 64 where they do not (192 of the 256 CUs); a plain product with too few tiles of either
+// size splits its contraction over about two blocks a CU, 4 k tiles each at least, and is joined by a second launch.
+struct GemmPlan { int tile, tiles_m, tiles_n, splits; };
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bool split) {
+    GemmPlan p;
+    auto tiles = [&](int t) {
+        p.tile = t;
+        p.tiles_m = (int)((M + t - 1) / t);
+        p.tiles_n = (int)(dual ? (N + t / 2 - 1) / (t / 2) : (N + t - 1) / t);
+        return (int64_t)p.tiles_m * p.tiles_n * z;
+    };
+    p.splits = 1;
+    const int64_t kt = (k + bk - 1) / bk;
+    int64_t n = tiles(128);
+    if (n >= 192 || (split && n * (kt / 4) >= 192)) {
+        if (split && n < 192) p.splits = (int)std::min<int64_t>(512 / n, kt / 4);
+        return p;
+    }
+    n = tiles(64);
+    if (split && n < 192) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / n, kt / 4));
+    return p;
+}
+
 template <typename T, bool PA, bool QA, int EPI>
-int gemm_launch(GemmArgs a, hipStream_t st) {
-    constexpr int BK = sizeof(T) == 4 ? 32 : 64, BM = 128, BN = 128, BNC = EPI == EPI_DUAL ? BN / 2 : BN;
-    a.tiles_m = (a.M + BM - 1) / BM;
-    a.tiles_n = (a.N + BNC - 1) / BNC;
-    const int64_t blocks = (int64_t)a.tiles_m * a.tiles_n * a.splits * a.z;
+int gemm_launch(GemmArgs a, float *ws, hipStream_t st) {
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    const GemmPlan p = gemm_plan(a.M, a.N, (int64_t)a.K * a.segs, a.z, BK, EPI == EPI_DUAL, EPI == EPI_PLAIN);
+    a.tiles_m = p.tiles_m;
+    a.tiles_n = p.tiles_n;
+    a.splits = p.splits;
+    a.parts = p.splits > 1 ? ws : nullptr;
+    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits * a.z;
     if (blocks > 0x7fffffff) return NMRF_EINVAL;
-    hipLaunchKernelGGL((ffn_gemm_kernel<T, BM, BN, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (p.tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (p.splits > 1) {
+        const int64_t n = (int64_t)a.M * a.N;
+        JoinArgs j{{ws, ws + p.splits * n, nullptr}, {a.C, a.C2, nullptr}, a.bias, {n, n, 0}, p.splits, a.N};
+        hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div64(n, 256), 4096), (unsigned)a.z), dim3(256), 0, st, j);
+    }
     return nmrf_launch_status();
+}
+// floats a plain product keeps in the workspace
+int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int z, int bk) {
+    const GemmPlan p = gemm_plan(M, N, k, z, bk, false, true);
+    return p.splits > 1 ? (int64_t)p.splits * z * M * N : 0;
 }
 
 struct FfnShape { int64_t T; int D, F, Do; };
@@ -565,19 +661,13 @@ bool ffn_misaligned(std::initializer_list<const void *> ps, int dtype) {
     for (const void *p : ps) o |= reinterpret_cast<uintptr_t>(p);
     return o & (dtype == NMRF_F32 ? 3 : 1);
 }
-int absmax(const float *const *p, const int64_t *n, const int *slot, int count, unsigned *amax, int zero, hipStream_t st) {
-    AbsmaxArgs a{};
-    for (int i = 0; i < count; ++i) { a.p[i] = p[i]; a.n[i] = n[i]; a.slot[i] = slot[i]; }
-    a.out = amax;
-    hipLaunchKernelGGL(ffn_zero_kernel, dim3(NSLOT), dim3(64), 0, st, amax, zero);
-    if (count) hipLaunchKernelGGL(ffn_absmax_kernel, dim3(256, (unsigned)count), dim3(256), 0, st, a);
-    return nmrf_launch_status();
-}
+int64_t colsum_blocks(int64_t T) { return T < 512 ? 1 : std::min<int64_t>(T / 256, 128); }
+constexpr int64_t FEW = 64;                                        // rows that stream the weights once
 
 template <typename T>
 int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *bg, const void *bu, const void *bd,
-                int act, void *h, void *g, void *u, void *y, unsigned *amax, hipStream_t st) {
-    if (s.T <= 64 && !g) {
+                int act, void *h, float *g, float *u, void *y, unsigned *amax, float *ws, hipStream_t st) {
+    if (s.T <= FEW && !g) {
         FewArgs f{x, wg, wu, bg, bu, h, (int)s.T, s.F, s.D, act, s.D, s.D, s.F};
         few_launch<T, 2>(f, st);
         FewArgs d{h, wd, wd, bd, nullptr, y, (int)s.T, s.Do, s.F, act, s.F, s.F, s.Do};
@@ -585,34 +675,25 @@ int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu
         return nmrf_launch_status();
     }
     if constexpr (sizeof(T) == 4) {
-        const float *p[4] = {(const float *)x, (const float *)wg, (const float *)wu, (const float *)wd};
-        const int64_t n[4] = {s.T * s.D, (int64_t)s.F * s.D, (int64_t)s.F * s.D, (int64_t)s.Do * s.F};
-        const int slot[4] = {SLOT_X, SLOT_W, SLOT_W, SLOT_WD};
-        const int rc = absmax(p, n, slot, 4, amax, 1 << SLOT_X | 1 << SLOT_W | 1 << SLOT_WD | 1 << SLOT_H, st);
-        if (rc != NMRF_OK) return rc;
+        AbsmaxArgs m{{(const float *)x, (const float *)wg, (const float *)wu, (const float *)wd, nullptr},
+                     {s.T * s.D, (int64_t)s.F * s.D, (int64_t)s.F * s.D, (int64_t)s.Do * s.F, 0},
+                     {SLOT_X, SLOT_WG, SLOT_WU, SLOT_WD, SLOT_H}, amax};
+        hipLaunchKernelGGL(ffn_absmax_kernel, dim3(256, 5), dim3(256), 0, st, m);
     }
     GemmArgs a{};
     a.P[0] = x; a.Q[0] = wg; a.Q[1] = wu; a.ldp = a.ldq = s.D; a.ldc = s.F;
-    a.M = (int)s.T; a.N = s.F; a.K = s.D; a.segs = 1; a.splits = 1; a.z = 1;
-    a.C = h; a.C2 = g; a.C3 = u; a.bias = bg; a.bias2 = bu; a.act = act; a.amax = amax; a.slot_p = SLOT_X; a.slot_q = SLOT_W; a.slot_out = SLOT_H;
-    int rc = gemm_launch<T, true, true, EPI_DUAL>(a, st);
+    a.M = (int)s.T; a.N = s.F; a.K = s.D; a.segs = 1; a.z = 1;
+    a.C = h; a.C2 = g; a.C3 = u; a.bias = bg; a.bias2 = bu; a.act = act; a.amax = amax; a.slot_p = SLOT_X; a.slot_q = SLOT_WG; a.slot_out = SLOT_H;
+    int rc = gemm_launch<T, true, true, EPI_DUAL>(a, nullptr, st);
     if (rc != NMRF_OK) return rc;
     GemmArgs b{};
     b.P[0] = h; b.Q[0] = wd; b.ldp = b.ldq = s.F; b.ldc = s.Do;
-    b.M = (int)s.T; b.N = s.Do; b.K = s.F; b.segs = 1; b.splits = 1; b.z = 1;
+    b.M = (int)s.T; b.N = s.Do; b.K = s.F; b.segs = 1; b.z = 1;
     b.C = y; b.bias = bd; b.amax = amax; b.slot_p = SLOT_H; b.slot_q = SLOT_WD; b.slot_out = -1;
-    return gemm_launch<T, true, true, EPI_PLAIN>(b, st);
+    return gemm_launch<T, true, true, EPI_PLAIN>(b, ws, st);
 }
 
-// weight gradient: z products P_z^T Q over all T tokens, the contraction split until the chip is full
-int wgrad_splits(int64_t T, int M, int N, int z, int bk) {
-    const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 127) / 128) * z, ktiles = (T + bk - 1) / bk;
-    int64_t s = tiles >= 384 ? 1 : 768 / tiles;
-    if (s > ktiles / 4) s = ktiles / 4;
-    return (int)(s < 1 ? 1 : s);
-}
-int64_t colsum_blocks(int64_t T) { return T < 2048 ? 1 : (T / 256 < 128 ? T / 256 : 128); }
-
+// weight gradient: one or two products P_z^T Q over all T tokens
 template <typename T>
 int wgrad(const void *p0, const void *p1, const void *q, int64_t tokens, int M, int N, void *c0, void *c1, float *ws, unsigned *amax, int slot_p, int slot_q,
           hipStream_t st) {
@@ -620,102 +701,110 @@ int wgrad(const void *p0, const void *p1, const void *q, int64_t tokens, int M, 
     a.P[0] = p0; a.P[1] = p1; a.Q[0] = q; a.ldp = M; a.ldq = N; a.ldc = N;
     a.M = M; a.N = N; a.K = (int)tokens; a.segs = 1; a.z = p1 ? 2 : 1;
     a.C = c0; a.C2 = c1; a.amax = amax; a.slot_p = slot_p; a.slot_q = slot_q; a.slot_out = -1;
-    a.splits = wgrad_splits(tokens, M, N, a.z, sizeof(T) == 4 ? 32 : 64);
-    a.parts = a.splits > 1 ? ws : nullptr;
-    const int rc = gemm_launch<T, false, false, EPI_PLAIN>(a, st);
-    if (rc != NMRF_OK || a.splits == 1) return rc;
-    const int64_t n = (int64_t)M * N;
-    int64_t blocks = ceil_div64(n, 1024);
-    if (blocks > 4096) blocks = 4096;
-    hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)blocks, (unsigned)a.z), dim3(256), 0, st, ws, a.splits, n, (T *)c0, (T *)c1);
-    return nmrf_launch_status();
-}
-template <typename T>
-int colsum(const void *x, int64_t tokens, int N, void *out, float *ws, hipStream_t st) {
-    const int64_t nb = colsum_blocks(tokens), rows = ceil_div64(tokens, nb);
-    hipLaunchKernelGGL(ffn_colsum_kernel<T>, dim3((unsigned)((N + 63) / 64), (unsigned)nb), dim3(256), 0, st, (const T *)x, tokens, N, rows, ws);
-    int64_t blocks = ceil_div64(N, 1024);
-    hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)blocks, 1), dim3(256), 0, st, ws, (int)nb, (int64_t)N, (T *)out, (T *)nullptr);
-    return nmrf_launch_status();
+    return gemm_launch<T, false, false, EPI_PLAIN>(a, ws, st);
 }
 
 template <typename T>
-int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *h, const void *g, const void *u, const void *dy,
-                 int act, void *dg, void *du, void *dx, void *dwg, void *dwu, void *dwd, void *dbg, void *dbu, void *dbd, unsigned *amax, float *ws,
-                 hipStream_t st) {
+int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *h, const float *g, const float *u,
+                 const void *dy, int act, void *dg, void *du, void *dx, void *dwg, void *dwu, void *dwd, void *dbg, void *dbu, void *dbd, unsigned *amax,
+                 float *ws, hipStream_t st) {
     int rc;
     if constexpr (sizeof(T) == 4) {
-        const float *p[1] = {(const float *)dy};
-        const int64_t n[1] = {s.T * s.Do};
-        const int slot[1] = {SLOT_DY};
-        if ((rc = absmax(p, n, slot, 1, amax, 1 << SLOT_DY | 1 << SLOT_DG, st)) != NMRF_OK) return rc;
+        AbsmaxArgs m{{(const float *)dy, nullptr}, {s.T * s.Do, 0}, {SLOT_DY, SLOT_DG}, amax};
+        hipLaunchKernelGGL(ffn_absmax_kernel, dim3(256, 2), dim3(256), 0, st, m);
     }
     GemmArgs a{};
     a.P[0] = dy; a.Q[0] = wd; a.ldp = s.Do; a.ldq = s.F; a.ldc = s.F;
-    a.M = (int)s.T; a.N = s.F; a.K = s.Do; a.segs = 1; a.splits = 1; a.z = 1;
+    a.M = (int)s.T; a.N = s.F; a.K = s.Do; a.segs = 1; a.z = 1;
     a.C = dg; a.C2 = du; a.g = g; a.u = u; a.act = act; a.amax = amax; a.slot_p = SLOT_DY; a.slot_q = SLOT_WD; a.slot_out = SLOT_DG;
-    if ((rc = gemm_launch<T, true, false, EPI_DH>(a, st)) != NMRF_OK) return rc;
+    if ((rc = gemm_launch<T, true, false, EPI_DH>(a, nullptr, st)) != NMRF_OK) return rc;
     if (dx) {
         GemmArgs b{};
         b.P[0] = dg; b.P[1] = du; b.Q[0] = wg; b.Q[1] = wu; b.ldp = s.F; b.ldq = s.D; b.ldc = s.D;
-        b.M = (int)s.T; b.N = s.D; b.K = s.F; b.segs = 2; b.splits = 1; b.z = 1;
-        b.C = dx; b.amax = amax; b.slot_p = SLOT_DG; b.slot_q = SLOT_W; b.slot_out = -1;
-        if ((rc = gemm_launch<T, true, false, EPI_PLAIN>(b, st)) != NMRF_OK) return rc;
+        b.M = (int)s.T; b.N = s.D; b.K = s.F; b.segs = 2; b.z = 1;
+        b.C = dx; b.amax = amax; b.slot_p = SLOT_DG; b.slot_q = SLOT_WG; b.slot_out = -1;
+        if ((rc = gemm_launch<T, true, false, EPI_PLAIN>(b, ws, st)) != NMRF_OK) return rc;
     }
-    if (dwg && dwu) {
-        if ((rc = wgrad<T>(dg, du, x, s.T, s.F, s.D, dwg, dwu, ws, amax, SLOT_DG, SLOT_X, st)) != NMRF_OK) return rc;
-    } else if (dwg || dwu) {
-        if ((rc = wgrad<T>(dwg ? dg : du, nullptr, x, s.T, s.F, s.D, dwg ? dwg : dwu, nullptr, ws, amax, SLOT_DG, SLOT_X, st)) != NMRF_OK) return rc;
+    if (dwg || dwu) {
+        const bool both = dwg && dwu;
+        rc = wgrad<T>(dwg ? dg : du, both ? du : nullptr, x, s.T, s.F, s.D, dwg ? dwg : dwu, both ? dwu : nullptr, ws, amax, SLOT_DG, SLOT_X, st);
+        if (rc != NMRF_OK) return rc;
     }
     if (dwd && (rc = wgrad<T>(dy, nullptr, h, s.T, s.Do, s.F, dwd, nullptr, ws, amax, SLOT_DY, SLOT_H, st)) != NMRF_OK) return rc;
-    if (dbg && (rc = colsum<T>(dg, s.T, s.F, dbg, ws, st)) != NMRF_OK) return rc;
-    if (dbu && (rc = colsum<T>(du, s.T, s.F, dbu, ws, st)) != NMRF_OK) return rc;
-    if (dbd && (rc = colsum<T>(dy, s.T, s.Do, dbd, ws, st)) != NMRF_OK) return rc;
-    return NMRF_OK;
+    // bias gradients: one launch of column sums, one join
+    const int64_t nb = colsum_blocks(s.T);
+    ColsumArgs c{};
+    JoinArgs j{};
+    int count = 0, widest = 0;
+    float *at = ws;
+    auto add = [&](const void *m, int cols, void *out) {
+        if (!out) return;
+        c.x[count] = m; c.cols[count] = cols; c.parts[count] = at;
+        j.parts[count] = at; j.c[count] = out; j.n[count++] = cols;
+        at += nb * cols;
+        widest = std::max(widest, cols);
+    };
+    add(dg, s.F, dbg);
+    add(du, s.F, dbu);
+    add(dy, s.Do, dbd);
+    if (count) {
+        c.rows = s.T;
+        c.per = ceil_div64(s.T, nb);
+        j.splits = (int)nb;
+        hipLaunchKernelGGL(ffn_colsum_kernel<T>, dim3((unsigned)((widest + 63) / 64), (unsigned)nb, (unsigned)count), dim3(256), 0, st, c);
+        hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)((widest + 255) / 256), (unsigned)count), dim3(256), 0, st, j);
+    }
+    return nmrf_launch_status();
 }
 
 }  // namespace
 
+extern "C" int nmrf_gated_ffn_size(int64_t T, int D, int F, int Do, int dtype, int backward, int64_t *floats) {
+    if (!floats) return NMRF_ENULL;
+    if (ffn_bad(FfnShape{T, D, F, Do}, dtype, 0)) return NMRF_EINVAL;
+    const int bk = dtype == NMRF_F32 ? 32 : 64;
+    int64_t n = T < 1 ? 0 : gemm_floats(T, backward ? D : Do, backward ? 2 * (int64_t)F : F, 1, bk);
+    if (backward && T > 0) {
+        for (int z = 1; z <= 2; ++z) n = std::max(n, gemm_floats(F, D, T, z, bk));
+        n = std::max(n, gemm_floats(Do, F, T, 1, bk));
+        n = std::max(n, colsum_blocks(T) * (2 * (int64_t)F + Do));
+    }
+    *floats = n;
+    return NMRF_OK;
+}
+
 extern "C" int nmrf_gated_ffn(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *b_gate, const void *b_up,
-                              const void *b_down, int64_t T, int D, int F, int Do, int dtype, int act, void *h, void *g, void *u, void *y,
-                              uint32_t *amax, void *stream) {
+                              const void *b_down, int64_t T, int D, int F, int Do, int dtype, int act, void *h, float *g, float *u, void *y,
+                              uint32_t *amax, float *ws, int64_t ws_floats, void *stream) {
     const FfnShape s{T, D, F, Do};
     if (ffn_bad(s, dtype, act)) return NMRF_EINVAL;
     if (T == 0) return NMRF_OK;
     if (!x || !w_gate || !w_up || !w_down || !h || !y || (dtype == NMRF_F32 && !amax)) return NMRF_ENULL;
-    if ((g == nullptr) != (u == nullptr) || ffn_misaligned({x, w_gate, w_up, w_down, b_gate, b_up, b_down, h, g, u, y}, dtype)) return NMRF_EINVAL;
-    if (reinterpret_cast<uintptr_t>(amax) & 3) return NMRF_EINVAL;
+    if ((g == nullptr) != (u == nullptr) || ffn_misaligned({x, w_gate, w_up, w_down, b_gate, b_up, b_down, h, y}, dtype)) return NMRF_EINVAL;
+    if (ffn_misaligned({amax, ws, g, u}, NMRF_F32)) return NMRF_EINVAL;
+    int64_t need = 0;
+    if (T > FEW || g) {
+        const int rc = nmrf_gated_ffn_size(T, D, F, Do, dtype, 0, &need);
+        if (rc != NMRF_OK || need > ws_floats) return NMRF_EINVAL;
+        if (need && !ws) return NMRF_ENULL;
+    }
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == NMRF_F32) return ffn_forward<float>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, st);
-    if (dtype == NMRF_BF16) return ffn_forward<__bf16>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, st);
-    return ffn_forward<_Float16>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, st);
+    if (dtype == NMRF_F32) return ffn_forward<float>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, ws, st);
+    if (dtype == NMRF_BF16) return ffn_forward<__bf16>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, ws, st);
+    return ffn_forward<_Float16>(s, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, h, g, u, y, amax, ws, st);
 }
 
-extern "C" int nmrf_gated_ffn_bwd_size(int64_t T, int D, int F, int Do, int dtype, int64_t *floats) {
-    if (!floats) return NMRF_ENULL;
-    if (ffn_bad(FfnShape{T, D, F, Do}, dtype, 0) || T < 1) return NMRF_EINVAL;
-    const int bk = dtype == NMRF_F32 ? 32 : 64;
-    int64_t n = 0;
-    const int s2 = wgrad_splits(T, F, D, 2, bk), s1 = wgrad_splits(T, F, D, 1, bk), sd = wgrad_splits(T, Do, F, 1, bk);
-    const int64_t a = s2 > 1 ? 2 * (int64_t)s2 * F * D : 0, b = s1 > 1 ? (int64_t)s1 * F * D : 0, c = sd > 1 ? (int64_t)sd * Do * F : 0;
-    n = a > b ? a : b;
-    n = n > c ? n : c;
-    const int64_t cs = colsum_blocks(T) * (int64_t)(F > Do ? F : Do);
-    *floats = n > cs ? n : cs;
-    return NMRF_OK;
-}
-
-extern "C" int nmrf_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const void *g, const void *u,
+extern "C" int nmrf_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *h, const float *g, const float *u,
                                   const void *dy, int64_t T, int D, int F, int Do, int dtype, int act, void *dg, void *du, void *dx, void *dw_gate,
                                   void *dw_up, void *dw_down, void *db_gate, void *db_up, void *db_down, uint32_t *amax, float *ws,
                                   int64_t ws_floats, void *stream) {
     const FfnShape s{T, D, F, Do};
     if (ffn_bad(s, dtype, act) || T < 1) return NMRF_EINVAL;
     if (!x || !w_gate || !w_up || !w_down || !h || !g || !u || !dy || !dg || !du || !ws || (dtype == NMRF_F32 && !amax)) return NMRF_ENULL;
-    if (ffn_misaligned({x, w_gate, w_up, w_down, h, g, u, dy, dg, du, dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down}, dtype)) return NMRF_EINVAL;
-    if ((reinterpret_cast<uintptr_t>(amax) | reinterpret_cast<uintptr_t>(ws)) & 3) return NMRF_EINVAL;
+    if (ffn_misaligned({x, w_gate, w_up, w_down, h, dy, dg, du, dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down}, dtype)) return NMRF_EINVAL;
+    if (ffn_misaligned({amax, ws, g, u}, NMRF_F32)) return NMRF_EINVAL;
     int64_t need = 0;
-    const int rc = nmrf_gated_ffn_bwd_size(T, D, F, Do, dtype, &need);
+    const int rc = nmrf_gated_ffn_size(T, D, F, Do, dtype, 1, &need);
     if (rc != NMRF_OK || need > ws_floats) return NMRF_EINVAL;
     hipStream_t st = (hipStream_t)stream;
 #define NMRF_FFN_BWD(TYPE) ffn_backward<TYPE>(s, x, w_gate, w_up, w_down, h, g, u, dy, act, dg, du, dx, dw_gate, dw_up, dw_down, db_gate, db_up, \

@@ -1568,16 +1568,23 @@ def residual_norm_backward(x, y, gate, scale, post_w, post_b, next_w, next_b, d_
     return [dx, dy] + grads
 
 
+def _ffn_workspace(x, f, do, backward):
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().nmrf_gated_ffn_size(x.shape[0], x.shape[1], f, do, DTYPE_CODE[x.dtype], backward, ctypes.byref(size)), "gated_ffn_size")
+    return (torch.empty(size.value, device=x.device, dtype=torch.float32) if size.value else None), size.value
+
+
 @_on_device
 def gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
     """x [T, D] -> (y, h, g, u, amax); g, u None without `keep` (the backward pass needs them), amax None for 16-bit types."""
     t, d = x.shape
     f, do = w_gate.shape[0], w_down.shape[0]
     y, h = x.new_empty(t, do), x.new_empty(t, f)
-    g, u = (x.new_empty(t, f), x.new_empty(t, f)) if keep else (None, None)
-    amax = torch.empty(384, device=x.device, dtype=torch.int32) if x.dtype == torch.float32 else None
+    g, u = (x.new_empty((2, t, f), dtype=torch.float32) if keep else (None, None))
+    amax = torch.empty(1792, device=x.device, dtype=torch.int32) if x.dtype == torch.float32 else None
+    ws, floats = _ffn_workspace(x, f, do, 0)
     _lib.check(_lib.load().nmrf_gated_ffn(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(b_gate), _p(b_up), _p(b_down), t, d, f, do, DTYPE_CODE[x.dtype],
-                                          act, _p(h), _p(g), _p(u), _p(y), _p(amax), _raw_stream()), "gated_ffn")
+                                          act, _p(h), _p(g), _p(u), _p(y), _p(amax), _p(ws), floats, _raw_stream()), "gated_ffn")
     return y, h, g, u, amax
 
 
@@ -1590,12 +1597,9 @@ def gated_ffn_backward(x, w_gate, w_up, w_down, h, g, u, amax, dy, act, want):
     if t == 0:
         return [x.new_zeros(s) if w else None for s, w in zip(shapes, want)]
     grads = [x.new_empty(s) if w else None for s, w in zip(shapes, want)]
-    dg, du = torch.empty_like(g), torch.empty_like(u)
-    size = ctypes.c_int64()
-    lib = _lib.load()
-    _lib.check(lib.nmrf_gated_ffn_bwd_size(t, d, f, do, DTYPE_CODE[x.dtype], ctypes.byref(size)), "gated_ffn_bwd")
-    ws = torch.empty(size.value, device=x.device, dtype=torch.float32)
+    dg, du = x.new_empty(2, t, f)
+    ws, floats = _ffn_workspace(x, f, do, 1)
     amax = None if amax is None else amax.clone()                      # (a second backward pass of one graph may run beside this one)
-    _lib.check(lib.nmrf_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(h), _p(g), _p(u), _p(dy), t, d, f, do, DTYPE_CODE[x.dtype], act,
-                                      _p(dg), _p(du), *[_p(v) for v in grads], _p(amax), _p(ws), ws.numel(), _raw_stream()), "gated_ffn_bwd")
+    _lib.check(_lib.load().nmrf_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(h), _p(g), _p(u), _p(dy), t, d, f, do, DTYPE_CODE[x.dtype],
+                                              act, _p(dg), _p(du), *[_p(v) for v in grads], _p(amax), _p(ws), floats, _raw_stream()), "gated_ffn_bwd")
     return grads

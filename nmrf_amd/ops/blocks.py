@@ -145,8 +145,8 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act=
     second matrix in another.
 
     x: [..., D]; w_gate, w_up: [F, D]; w_down: [D', F]; biases [F], [F], [D'], each may be None; one type, fp32 / bf16 / fp16 (copied where not
-    contiguous).  act: "silu", "gelu" (erf) or "relu".  16-bit types multiply on the matrix pipe as they are (sums in fp32; h and, for the
-    backward pass, both projections are kept in the type); fp32 is multiplied as scaled fp16 pairs: errors of 2^-22 relative to each operand's
+    contiguous).  act: "silu", "gelu" (erf) or "relu".  16-bit types multiply on the matrix pipe as they are (sums in fp32; h is kept in the
+    type, both projections for the backward pass in fp32); fp32 is multiplied as scaled fp16 pairs: errors of 2^-22 relative to each operand's
     largest entry, and an infinite input gives NaN.  Differentiable in every tensor, the same bits every run.  Up to 64 rows without gradients
     (decoding) stream the weights once.  The forward pass may be captured into a graph, the backward pass may not (it raises)."""
     if act not in _FFN_ACTS:

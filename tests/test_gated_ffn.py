@@ -110,12 +110,12 @@ def test_refusals():
 def test_c_entries_refuse_before_they_launch():
     lib = _lib.load()
 
-    def fwd(x=64, t=4, d=8, f=8, do=8, dtype=1, act=0, h=64, g=None, u=None, y=64, amax=None):
-        return lib.nmrf_gated_ffn(x, 64, 64, 64, None, None, None, t, d, f, do, dtype, act, h, g, u, y, amax, None)
+    def fwd(x=64, t=4, d=8, f=8, do=8, dtype=1, act=0, h=64, g=None, u=None, y=64, amax=None, ws=64, floats=1 << 30):
+        return lib.nmrf_gated_ffn(x, 64, 64, 64, None, None, None, t, d, f, do, dtype, act, h, g, u, y, amax, ws, floats, None)
     assert fwd(t=0) == 0
     assert fwd(x=None) == -3 and fwd(h=None) == -3 and fwd(y=None) == -3 and fwd(dtype=0) == -3
     for bad in (dict(t=-1), dict(d=0), dict(f=0), dict(do=0), dict(d=(1 << 22) + 1), dict(dtype=3), dict(act=3), dict(g=64), dict(x=65), dict(y=65),
-                dict(x=66, dtype=0, amax=64), dict(dtype=0, amax=66), dict(t=0x7fffffff)):
+                dict(x=66, dtype=0, amax=64), dict(dtype=0, amax=66), dict(t=0x7fffffff), dict(g=66, u=64), dict(ws=66), dict(t=200, f=8192, floats=0)):
         assert fwd(**bad) == -1, bad
 
     def bwd(t=4, dtype=1, ws=64, floats=1 << 30, dg=64, amax=None):
@@ -123,13 +123,15 @@ def test_c_entries_refuse_before_they_launch():
     assert bwd(t=0) == -1 and bwd(ws=None) == -3 and bwd(dg=None) == -3 and bwd(dtype=0) == -3 and bwd(floats=0) == -1 and bwd(ws=66) == -1 and bwd(dg=65) == -1
     import ctypes
     n = ctypes.c_int64()
-    assert lib.nmrf_gated_ffn_bwd_size(0, 8, 8, 8, 0, ctypes.byref(n)) == -1 and lib.nmrf_gated_ffn_bwd_size(4, 8, 8, 8, 0, None) == -3
-    assert lib.nmrf_gated_ffn_bwd_size(29952, 128, 512, 128, 0, ctypes.byref(n)) == 0 and n.value > 2 * 128 * 512
+    size = lambda t, back, p=ctypes.byref(n): lib.nmrf_gated_ffn_size(t, 128, 512, 128, 0, back, p)  # noqa: E731
+    assert size(-1, 1) == -1 and size(4, 1, None) == -3 and size(0, 1) == 0 and n.value == 0
+    assert size(29952, 1) == 0 and n.value > 2 * 128 * 512 and size(29952, 0) == 0 and n.value == 0
 
 
 # ---- the formula ------------------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (3, 17, 33, 5), (16, 64, 128, 64), (17, 40, 72, 24), (64, 96, 200, 96), (65, 128, 64, 128), (127, 33, 129, 65),
-          (128, 128, 128, 128), (129, 136, 264, 72), (300, 321, 861, 321), (777, 64, 100, 48), (1000, 128, 512, 128), (5000, 72, 136, 40)]
+          (128, 128, 128, 128), (129, 136, 264, 72), (300, 321, 861, 321), (777, 64, 100, 48), (1000, 128, 512, 128), (5000, 72, 136, 40),
+          (200, 1, 3, 2), (321, 3, 1, 7), (2100, 200, 130, 9), (450, 700, 1030, 60)]
 
 
 @pytest.mark.gpu
