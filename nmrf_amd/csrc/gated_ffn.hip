@@ -105,17 +105,22 @@ __device__ __forceinline__ int slot_shift(const unsigned *amax, int slot, int co
 //     C[m, n] = sum over segments s and k of P_s[m, k] Q_s[n, k]
 // An operand lies ALONG k (row m: k contiguous, stride ld) or ACROSS it (row k: m contiguous, stride ld).
 enum { EPI_DUAL = 0, EPI_PLAIN = 1, EPI_DH = 2 };
-struct GemmArgs {
-    const void *P[2], *Q[2];
+struct Problem {
+    const void *P[2], *Q[2];                     // the segments of a contraction (EPI_DUAL: Q = Wg, Wu)
     int64_t ldp, ldq, ldc;
     int M, N, K, segs;                           // K of one segment
     void *C, *C2, *C3;                           // EPI_DUAL: h, g, u (C2, C3 fp32, may be null); EPI_PLAIN: the product; EPI_DH: dg, du in C, C2
     const float *g, *u;                          // EPI_DH
     const void *bias, *bias2;
     float *parts;                                // EPI_PLAIN with splits > 1: fp32 partial products [splits][M][N]
-    unsigned *amax;                              // fp32: the slots above
-    int slot_p, slot_q, slot_out;                // slot_out: where the largest magnitude of the output goes (-1: nowhere)
-    int act, splits, tiles_m, tiles_n, z;        // z problems side by side (P[z], C / C2): the two weight gradients of dg and du
+    float *sum1, *sum2;                          // EPI_DH: column sums of dg, du over each wave's rows, [2 tiles_m][N] (may be null)
+    int slot_p, slot_q, slot_out;                // fp32: slots of the operands' and the output's largest magnitudes (slot_out -1: none)
+    int splits, tiles_m, tiles_n, blocks;
+};
+struct GemmArgs {
+    Problem p[3];                                // side by side in one launch
+    int count, act;
+    unsigned *amax;
 };
 
 template <typename T, int ROWS, int BK, bool ALONG, int THREADS> struct Stage {
@@ -197,21 +202,20 @@ template <typename T, int ROWS, int BK, bool ALONG, int THREADS> struct Stage {
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int BK, bool PA, bool QA, int EPI>
-__global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
     using H = Half<T>;
     constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, PL = sizeof(T) == 4 ? 2 : 1;
     using SP = Stage<T, BM, BK, PA, THREADS>;
     using SQ = Stage<T, BN, BK, QA, THREADS>;
     __shared__ __align__(16) H lds[2][PL * (BM + BN) * BK];
+    int bid = blockIdx.x, which = 0;
+    while (which + 1 < args.count && bid >= args.p[which].blocks) bid -= args.p[which++].blocks;
+    const Problem &a = args.p[which];
     // blocks go to the 8 XCDs in turn: give each one a run of neighbouring tiles (its L2 then holds their operands), 8 row tiles deep
-    const int per_z = a.tiles_m * a.tiles_n, all = per_z * a.splits * a.z;
-    int t;
-    {
-        const int xcd = blockIdx.x & 7, q = all >> 3, rem = all & 7;
-        t = xcd * q + min(xcd, rem) + (blockIdx.x >> 3);
-    }
-    const int zz = t / (per_z * a.splits), sp = t / per_z % a.splits;
-    t %= per_z;
+    const int per_split = a.tiles_m * a.tiles_n, q8 = a.blocks >> 3, rem = a.blocks & 7, xcd = bid & 7;
+    int t = xcd * q8 + min(xcd, rem) + (bid >> 3);
+    const int sp = t / per_split;
+    t -= sp * per_split;
     const int band = t / (8 * a.tiles_n), deep = min(8, a.tiles_m - band * 8), in_band = t - band * 8 * a.tiles_n;
     const int tm = band * 8 + in_band % deep, tn = in_band / deep;
     constexpr int BNC = EPI == EPI_DUAL ? BN / 2 : BN;             // columns of the result
@@ -221,7 +225,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     float pmul = 1.f, qmul = 1.f;
     int unshift = 0;
     if constexpr (PL == 2) {
-        const int sp_ = slot_shift(a.amax, a.slot_p, 1), sq_ = slot_shift(a.amax, a.slot_q, a.slot_q == SLOT_WG ? 2 : 1);
+        const int sp_ = slot_shift(args.amax, a.slot_p, 1), sq_ = slot_shift(args.amax, a.slot_q, a.slot_q == SLOT_WG ? 2 : 1);
         pmul = ldexpf(1.f, sp_);
         qmul = ldexpf(1.f, sq_);
         unshift = -(sp_ + sq_);
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     SQ sQ;
     auto fetch = [&](int kt) {
         const int seg = kt / ktiles_seg, k0 = (kt - seg * ktiles_seg) * BK, left = a.K - k0;
-        const T *P = static_cast<const T *>((a.z > 1 ? zz : seg) ? a.P[1] : a.P[0]);
+        const T *P = static_cast<const T *>(seg ? a.P[1] : a.P[0]);
         const T *Q = static_cast<const T *>(EPI != EPI_DUAL && seg ? a.Q[1] : a.Q[0]);
         auto none = [](int, const T *&) { return (const T *)nullptr; };
         if constexpr (PA) {
@@ -342,13 +346,14 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
             for (int k = 0; k < 4; ++k) v[k] = k < left ? (float)p[k] : 0.f;
         }
     };
+    constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = m0 + (wm * TM + i) * 16 + (lane & 15);
-        constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN;
+    for (int j = 0; j < JN; ++j) {
+        const int n = n0 + (wn * JN + j) * 16 + 4 * (lane >> 4), left = a.N - n;
+        float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < JN; ++j) {
-            const int n = n0 + (wn * JN + j) * 16 + 4 * (lane >> 4), left = a.N - n;
+        for (int i = 0; i < TM; ++i) {
+            const int m = m0 + (wm * TM + i) * 16 + (lane & 15);
             if (m >= a.M || left <= 0) continue;
             const int64_t at = (int64_t)m * a.ldc + n;
             float v[4], w[4];
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    v[k] = act_value(v[k], a.act) * w[k];
+                    v[k] = act_value(v[k], args.act) * w[k];
                     if (k < left) top = fmaxf(top, fabsf(v[k]));
                 }
                 put4(a.C, at, left, v);
@@ -386,16 +391,21 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float value, slope;
-                    act_both(g[k], a.act, value, slope);
+                    act_both(g[k], args.act, value, slope);
                     w[k] = v[k] * value;
                     v[k] = v[k] * u[k] * slope;
                     if (k < left) top = fmaxf(top, fmaxf(fabsf(v[k]), fabsf(w[k])));
                 }
                 put4(a.C, at, left, v);
                 put4(a.C2, at, left, w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s1[k] += v[k];
+                    s2[k] += w[k];
+                }
             } else {
                 if (a.parts) {
-                    putf(a.parts + ((int64_t)(zz * a.splits + sp) * a.M + m) * a.N + n, left, v);
+                    putf(a.parts + ((int64_t)sp * a.M + m) * a.N + n, left, v);
                 } else {
                     if (a.bias) {
                         float b[4];
@@ -403,7 +413,27 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) v[k] += b[k];
                     }
-                    put4(zz ? a.C2 : a.C, at, left, v);
+                    put4(a.C, at, left, v);
+                }
+            }
+        }
+        if constexpr (EPI == EPI_DH) {
+            if (a.sum1 || a.sum2) {                                // bias gradients: over the wave's rows, 16 lanes of a row group
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s1[k] += NMRF_ROW_ROR(s1[k], 8);
+                    s2[k] += NMRF_ROW_ROR(s2[k], 8);
+                    s1[k] += NMRF_ROW_ROR(s1[k], 4);
+                    s2[k] += NMRF_ROW_ROR(s2[k], 4);
+                    s1[k] += NMRF_ROW_ROR(s1[k], 2);
+                    s2[k] += NMRF_ROW_ROR(s2[k], 2);
+                    s1[k] += NMRF_ROW_ROR(s1[k], 1);
+                    s2[k] += NMRF_ROW_ROR(s2[k], 1);
+                }
+                if ((lane & 15) == 0 && left > 0) {
+                    const int64_t at = (int64_t)(tm * WM + wm) * a.N + n;
+                    if (a.sum1) putf(a.sum1 + at, left, s1);
+                    if (a.sum2) putf(a.sum2 + at, left, s2);
                 }
             }
         }
@@ -411,41 +441,45 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs a) {
     if constexpr (PL == 2 && EPI != EPI_PLAIN) {
         if (a.slot_out >= 0) {
             top = wave_max(top);
-            if (lane == 0) atomicMax(a.amax + a.slot_out * 256 + (blockIdx.x & 255), __float_as_uint(top));
+            if (lane == 0) atomicMax(args.amax + a.slot_out * 256 + (blockIdx.x & 255), __float_as_uint(top));
         }
     }
 }
 
-// partial products [z][splits][n] -> the products (plus a bias of `cols` values): a block owns 256 values; its 4 row lanes add the splits l, l + 4,
-// ... in ascending order and the lane sums in ascending order
-struct JoinArgs { const float *parts[3]; void *c[3]; const void *bias; int64_t n[3]; int splits, cols; };
+// partial results [splits][n] -> the results (the first one plus a bias of `cols` values), several in one launch: a block owns 256 values; its 4
+// row lanes add the splits l, l + 4, ... in ascending order and the lane sums in ascending order
+struct JoinArgs { const float *parts[7]; void *c[7]; int64_t n[7]; int splits[7], blocks[7]; const void *bias; int cols, count; };
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_join_kernel(JoinArgs a) {
     __shared__ float sh[4][256];
-    const int64_t n = a.n[blockIdx.y];
-    const float *p = a.parts[blockIdx.y];
-    T *c = static_cast<T *>(a.c[blockIdx.y]);
+    int bid = blockIdx.x, which = 0;
+    while (which + 1 < a.count && bid >= a.blocks[which]) bid -= a.blocks[which++];
+    const int64_t n = a.n[which];
+    const int splits = a.splits[which], blocks = a.blocks[which];
+    const float *p = a.parts[which];
+    T *c = static_cast<T *>(a.c[which]);
+    const void *bias = which ? nullptr : a.bias;
     const int l = threadIdx.x >> 6;
-    for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n; i0 += (int64_t)gridDim.x * 256) {
+    for (int64_t i0 = (int64_t)bid * 256; i0 < n; i0 += (int64_t)blocks * 256) {
         const int64_t i = i0 + (threadIdx.x & 63) * 4;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
         if (i + 4 <= n) {
             int k = l;
-            for (; k + 12 < a.splits; k += 16) {                   // four loads in flight
+            for (; k + 12 < splits; k += 16) {                   // four loads in flight
                 float v[4][4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)(k + 4 * q) * n + i), v[q]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
             }
-            for (; k < a.splits; k += 4) {
+            for (; k < splits; k += 4) {
                 float v[4];
                 Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)k * n + i), v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += v[e];
             }
         } else {
-            for (int k = l; k < a.splits; k += 4)
+            for (int k = l; k < splits; k += 4)
                 for (int e = 0; e < 4; ++e)
                     if (i + e < n) s[e] += p[(int64_t)k * n + i + e];
         }
@@ -456,21 +490,20 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(JoinArgs a) {
         const int64_t j = i0 + threadIdx.x;
         if (j < n) {
             float v = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
-            if (a.bias) v += (float)static_cast<const T *>(a.bias)[j % a.cols];
+            if (bias) v += (float)static_cast<const T *>(bias)[j % a.cols];
             c[j] = (T)v;
         }
     }
 }
 
-// column sums (bias gradients) of up to three matrices of T rows: a block adds its rows of 64 columns (16 row lanes of 16 column lanes), a join
-// adds the blocks' partials
-struct ColsumArgs { const void *x[3]; float *parts[3]; int cols[3]; int64_t rows, per; };
+// column sums of dy (dg's and du's come out of the kernel that makes them): a block adds its rows of 64 columns (16 row lanes of 16 column
+// lanes), a join adds the blocks' partials
+struct ColsumArgs { const void *x; float *parts; int cols; int64_t rows, per; };
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_colsum_kernel(ColsumArgs a) {
     __shared__ float sh[16][65];
-    const int N = a.cols[blockIdx.z], c = blockIdx.x * 64 + (threadIdx.x & 15) * 4, l = threadIdx.x >> 4;
-    if (blockIdx.x * 64 >= N) return;
-    const T *x = static_cast<const T *>(a.x[blockIdx.z]);
+    const int N = a.cols, c = blockIdx.x * 64 + (threadIdx.x & 15) * 4, l = threadIdx.x >> 4;
+    const T *x = static_cast<const T *>(a.x);
     const int64_t r0 = blockIdx.y * a.per, r1 = min(a.rows, r0 + a.per);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c + 4 <= N) {
@@ -499,7 +532,7 @@ __global__ __launch_bounds__(256) void ffn_colsum_kernel(ColsumArgs a) {
         float v = sh[0][threadIdx.x];
 #pragma unroll
         for (int k = 1; k < 16; ++k) v += sh[k][threadIdx.x];
-        a.parts[blockIdx.z][(int64_t)blockIdx.y * N + blockIdx.x * 64 + threadIdx.x] = v;
+        a.parts[(int64_t)blockIdx.y * N + blockIdx.x * 64 + threadIdx.x] = v;
     }
 }
 
@@ -605,7 +638,8 @@ void few_launch(const FewArgs &a, hipStream_t st) {
 // Tiles of 128 x 128 where they fill the chip, of 64 x 64 where they do not (192 of the 256 CUs); a plain product with too few tiles of either
 // size splits its contraction over about two blocks a CU, 4 k tiles each at least, and is joined by a second launch.
 struct GemmPlan { int tile, tiles_m, tiles_n, splits; };
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bool split) {
+// z: problems in the launch; tile: that of the launch, 0: to be chosen
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bool split, int tile) {
     GemmPlan p;
     auto tiles = [&](int t) {
         p.tile = t;
@@ -613,41 +647,69 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bo
         p.tiles_n = (int)(dual ? (N + t / 2 - 1) / (t / 2) : (N + t - 1) / t);
         return (int64_t)p.tiles_m * p.tiles_n * z;
     };
-    p.splits = 1;
     const int64_t kt = (k + bk - 1) / bk;
-    int64_t n = tiles(128);
-    if (n >= 192 || (split && n * (kt / 4) >= 192)) {
-        if (split && n < 192) p.splits = (int)std::min<int64_t>(512 / n, kt / 4);
-        return p;
-    }
-    n = tiles(64);
-    if (split && n < 192) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / n, kt / 4));
+    int64_t n = tiles(tile ? tile : 128);
+    if (!tile && n < 192 && !(split && n * (kt / 4) >= 192)) n = tiles(64);
+    p.splits = split && n < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(512 / n, kt / 4)) : 1;
     return p;
 }
 
-template <typename T, bool PA, bool QA, int EPI>
-int gemm_launch(GemmArgs a, float *ws, hipStream_t st) {
-    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
-    const GemmPlan p = gemm_plan(a.M, a.N, (int64_t)a.K * a.segs, a.z, BK, EPI == EPI_DUAL, EPI == EPI_PLAIN);
-    a.tiles_m = p.tiles_m;
-    a.tiles_n = p.tiles_n;
-    a.splits = p.splits;
-    a.parts = p.splits > 1 ? ws : nullptr;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits * a.z;
-    if (blocks > 0x7fffffff) return NMRF_EINVAL;
-    if (p.tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    if (p.splits > 1) {
-        const int64_t n = (int64_t)a.M * a.N;
-        JoinArgs j{{ws, ws + p.splits * n, nullptr}, {a.C, a.C2, nullptr}, a.bias, {n, n, 0}, p.splits, a.N};
-        hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div64(n, 256), 4096), (unsigned)a.z), dim3(256), 0, st, j);
+// the outputs that wait for the join at the end of a pass, and the workspace behind them
+struct Pending {
+    JoinArgs j{};
+    float *ws;
+    explicit Pending(float *w) : ws(w) {}
+    float *add(int64_t n, int splits, void *c) {
+        float *at = ws;
+        const int k = j.count++;
+        j.parts[k] = at;
+        j.c[k] = c;
+        j.n[k] = n;
+        j.splits[k] = splits;
+        j.blocks[k] = (int)std::min<int64_t>(ceil_div64(n, 256), 4096);
+        ws += (int64_t)splits * n;
+        return at;
     }
+    template <typename T> int go(hipStream_t st) {
+        if (!j.count) return NMRF_OK;
+        unsigned blocks = 0;
+        for (int k = 0; k < j.count; ++k) blocks += (unsigned)j.blocks[k];
+        hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, st, j);
+        return nmrf_launch_status();
+    }
+};
+
+template <typename T, bool PA, bool QA, int EPI>
+int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    int tile = 0;
+    int64_t blocks = 0;
+    for (int i = 0; i < a.count; ++i) {
+        Problem &q = a.p[i];
+        const GemmPlan p = gemm_plan(q.M, q.N, (int64_t)q.K * q.segs, a.count, BK, EPI == EPI_DUAL, EPI == EPI_PLAIN, tile);
+        tile = p.tile;                                             // (problems of one launch share the first one's tile)
+        q.tiles_m = p.tiles_m;
+        q.tiles_n = p.tiles_n;
+        q.splits = p.splits;
+        q.parts = p.splits > 1 ? wait.add((int64_t)q.M * q.N, p.splits, q.C) : nullptr;
+        const int64_t n = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+        blocks += n;
+        if (blocks > 0x7fffffff) return NMRF_EINVAL;
+        q.blocks = (int)n;
+    }
+    if (tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     return nmrf_launch_status();
 }
-// floats a plain product keeps in the workspace
-int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int z, int bk) {
-    const GemmPlan p = gemm_plan(M, N, k, z, bk, false, true);
-    return p.splits > 1 ? (int64_t)p.splits * z * M * N : 0;
+// floats a plain product keeps in the workspace, at most (whatever shares its launch)
+int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int bk) {
+    int64_t n = 0;
+    for (int z = 1; z <= 3; ++z)
+        for (int tile = 0; tile <= 128; tile += 64) {
+            const int s = gemm_plan(M, N, k, z, bk, false, true, tile).splits;
+            n = std::max(n, s > 1 ? (int64_t)s * M * N : 0);
+        }
+    return n;
 }
 
 struct FfnShape { int64_t T; int D, F, Do; };
@@ -680,81 +742,73 @@ int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu
                      {SLOT_X, SLOT_WG, SLOT_WU, SLOT_WD, SLOT_H}, amax};
         hipLaunchKernelGGL(ffn_absmax_kernel, dim3(256, 5), dim3(256), 0, st, m);
     }
+    Pending wait(ws);
     GemmArgs a{};
-    a.P[0] = x; a.Q[0] = wg; a.Q[1] = wu; a.ldp = a.ldq = s.D; a.ldc = s.F;
-    a.M = (int)s.T; a.N = s.F; a.K = s.D; a.segs = 1; a.z = 1;
-    a.C = h; a.C2 = g; a.C3 = u; a.bias = bg; a.bias2 = bu; a.act = act; a.amax = amax; a.slot_p = SLOT_X; a.slot_q = SLOT_WG; a.slot_out = SLOT_H;
-    int rc = gemm_launch<T, true, true, EPI_DUAL>(a, nullptr, st);
+    a.count = 1; a.act = act; a.amax = amax;
+    Problem &p = a.p[0];
+    p.P[0] = x; p.Q[0] = wg; p.Q[1] = wu; p.ldp = p.ldq = s.D; p.ldc = s.F;
+    p.M = (int)s.T; p.N = s.F; p.K = s.D; p.segs = 1;
+    p.C = h; p.C2 = g; p.C3 = u; p.bias = bg; p.bias2 = bu; p.slot_p = SLOT_X; p.slot_q = SLOT_WG; p.slot_out = SLOT_H;
+    int rc = gemm_launch<T, true, true, EPI_DUAL>(a, wait, st);
     if (rc != NMRF_OK) return rc;
-    GemmArgs b{};
-    b.P[0] = h; b.Q[0] = wd; b.ldp = b.ldq = s.F; b.ldc = s.Do;
-    b.M = (int)s.T; b.N = s.Do; b.K = s.F; b.segs = 1; b.z = 1;
-    b.C = y; b.bias = bd; b.amax = amax; b.slot_p = SLOT_H; b.slot_q = SLOT_WD; b.slot_out = -1;
-    return gemm_launch<T, true, true, EPI_PLAIN>(b, ws, st);
-}
-
-// weight gradient: one or two products P_z^T Q over all T tokens
-template <typename T>
-int wgrad(const void *p0, const void *p1, const void *q, int64_t tokens, int M, int N, void *c0, void *c1, float *ws, unsigned *amax, int slot_p, int slot_q,
-          hipStream_t st) {
-    GemmArgs a{};
-    a.P[0] = p0; a.P[1] = p1; a.Q[0] = q; a.ldp = M; a.ldq = N; a.ldc = N;
-    a.M = M; a.N = N; a.K = (int)tokens; a.segs = 1; a.z = p1 ? 2 : 1;
-    a.C = c0; a.C2 = c1; a.amax = amax; a.slot_p = slot_p; a.slot_q = slot_q; a.slot_out = -1;
-    return gemm_launch<T, false, false, EPI_PLAIN>(a, ws, st);
+    p = Problem{};
+    p.P[0] = h; p.Q[0] = wd; p.ldp = p.ldq = s.F; p.ldc = s.Do;
+    p.M = (int)s.T; p.N = s.Do; p.K = s.F; p.segs = 1;
+    p.C = y; p.bias = bd; p.slot_p = SLOT_H; p.slot_q = SLOT_WD; p.slot_out = -1;
+    if ((rc = gemm_launch<T, true, true, EPI_PLAIN>(a, wait, st)) != NMRF_OK) return rc;
+    wait.j.bias = bd;
+    wait.j.cols = s.Do;
+    return wait.go<T>(st);
 }
 
 template <typename T>
 int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *h, const float *g, const float *u,
                  const void *dy, int act, void *dg, void *du, void *dx, void *dwg, void *dwu, void *dwd, void *dbg, void *dbu, void *dbd, unsigned *amax,
                  float *ws, hipStream_t st) {
+    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
     int rc;
     if constexpr (sizeof(T) == 4) {
         AbsmaxArgs m{{(const float *)dy, nullptr}, {s.T * s.Do, 0}, {SLOT_DY, SLOT_DG}, amax};
         hipLaunchKernelGGL(ffn_absmax_kernel, dim3(256, 2), dim3(256), 0, st, m);
     }
+    Pending wait(ws);
     GemmArgs a{};
-    a.P[0] = dy; a.Q[0] = wd; a.ldp = s.Do; a.ldq = s.F; a.ldc = s.F;
-    a.M = (int)s.T; a.N = s.F; a.K = s.Do; a.segs = 1; a.z = 1;
-    a.C = dg; a.C2 = du; a.g = g; a.u = u; a.act = act; a.amax = amax; a.slot_p = SLOT_DY; a.slot_q = SLOT_WD; a.slot_out = SLOT_DG;
-    if ((rc = gemm_launch<T, true, false, EPI_DH>(a, nullptr, st)) != NMRF_OK) return rc;
+    a.count = 1; a.act = act; a.amax = amax;
+    Problem &p = a.p[0];
+    p.P[0] = dy; p.Q[0] = wd; p.ldp = s.Do; p.ldq = s.F; p.ldc = s.F;
+    p.M = (int)s.T; p.N = s.F; p.K = s.Do; p.segs = 1;
+    p.C = dg; p.C2 = du; p.g = g; p.u = u; p.slot_p = SLOT_DY; p.slot_q = SLOT_WD; p.slot_out = SLOT_DG;
+    const int sums = 2 * gemm_plan(s.T, s.F, s.Do, 1, BK, false, false, 0).tiles_m;
+    if (dbg) p.sum1 = wait.add(s.F, sums, dbg);
+    if (dbu) p.sum2 = wait.add(s.F, sums, dbu);
+    if ((rc = gemm_launch<T, true, false, EPI_DH>(a, wait, st)) != NMRF_OK) return rc;
     if (dx) {
-        GemmArgs b{};
-        b.P[0] = dg; b.P[1] = du; b.Q[0] = wg; b.Q[1] = wu; b.ldp = s.F; b.ldq = s.D; b.ldc = s.D;
-        b.M = (int)s.T; b.N = s.D; b.K = s.F; b.segs = 2; b.z = 1;
-        b.C = dx; b.amax = amax; b.slot_p = SLOT_DG; b.slot_q = SLOT_WG; b.slot_out = -1;
-        if ((rc = gemm_launch<T, true, false, EPI_PLAIN>(b, ws, st)) != NMRF_OK) return rc;
+        p = Problem{};
+        p.P[0] = dg; p.P[1] = du; p.Q[0] = wg; p.Q[1] = wu; p.ldp = s.F; p.ldq = s.D; p.ldc = s.D;
+        p.M = (int)s.T; p.N = s.D; p.K = s.F; p.segs = 2;
+        p.C = dx; p.slot_p = SLOT_DG; p.slot_q = SLOT_WG; p.slot_out = -1;
+        if ((rc = gemm_launch<T, true, false, EPI_PLAIN>(a, wait, st)) != NMRF_OK) return rc;
     }
-    if (dwg || dwu) {
-        const bool both = dwg && dwu;
-        rc = wgrad<T>(dwg ? dg : du, both ? du : nullptr, x, s.T, s.F, s.D, dwg ? dwg : dwu, both ? dwu : nullptr, ws, amax, SLOT_DG, SLOT_X, st);
-        if (rc != NMRF_OK) return rc;
-    }
-    if (dwd && (rc = wgrad<T>(dy, nullptr, h, s.T, s.Do, s.F, dwd, nullptr, ws, amax, SLOT_DY, SLOT_H, st)) != NMRF_OK) return rc;
-    // bias gradients: one launch of column sums, one join
-    const int64_t nb = colsum_blocks(s.T);
-    ColsumArgs c{};
-    JoinArgs j{};
-    int count = 0, widest = 0;
-    float *at = ws;
-    auto add = [&](const void *m, int cols, void *out) {
-        if (!out) return;
-        c.x[count] = m; c.cols[count] = cols; c.parts[count] = at;
-        j.parts[count] = at; j.c[count] = out; j.n[count++] = cols;
-        at += nb * cols;
-        widest = std::max(widest, cols);
+    // weight gradients: products P^T Q over all T tokens, in one launch
+    a.count = 0;
+    auto wgrad = [&](const void *pp, const void *qq, int M, int N, void *c, int slot_p, int slot_q) {
+        if (!c) return;
+        Problem &w = a.p[a.count++];
+        w = Problem{};
+        w.P[0] = pp; w.Q[0] = qq; w.ldp = M; w.ldq = N; w.ldc = N;
+        w.M = M; w.N = N; w.K = (int)s.T; w.segs = 1;
+        w.C = c; w.slot_p = slot_p; w.slot_q = slot_q; w.slot_out = -1;
     };
-    add(dg, s.F, dbg);
-    add(du, s.F, dbu);
-    add(dy, s.Do, dbd);
-    if (count) {
-        c.rows = s.T;
-        c.per = ceil_div64(s.T, nb);
-        j.splits = (int)nb;
-        hipLaunchKernelGGL(ffn_colsum_kernel<T>, dim3((unsigned)((widest + 63) / 64), (unsigned)nb, (unsigned)count), dim3(256), 0, st, c);
-        hipLaunchKernelGGL(ffn_join_kernel<T>, dim3((unsigned)((widest + 255) / 256), (unsigned)count), dim3(256), 0, st, j);
+    wgrad(dg, x, s.F, s.D, dwg, SLOT_DG, SLOT_X);
+    wgrad(du, x, s.F, s.D, dwu, SLOT_DG, SLOT_X);
+    wgrad(dy, h, s.Do, s.F, dwd, SLOT_DY, SLOT_H);
+    if (a.count && (rc = gemm_launch<T, false, false, EPI_PLAIN>(a, wait, st)) != NMRF_OK) return rc;
+    if (dbd) {
+        const int64_t nb = colsum_blocks(s.T);
+        ColsumArgs c{dy, wait.add(s.Do, (int)nb, dbd), s.Do, s.T, ceil_div64(s.T, nb)};
+        hipLaunchKernelGGL(ffn_colsum_kernel<T>, dim3((unsigned)((s.Do + 63) / 64), (unsigned)nb), dim3(256), 0, st, c);
     }
-    return nmrf_launch_status();
+    return wait.go<T>(st);
 }
 
 }  // namespace
@@ -763,12 +817,11 @@ extern "C" int nmrf_gated_ffn_size(int64_t T, int D, int F, int Do, int dtype, i
     if (!floats) return NMRF_ENULL;
     if (ffn_bad(FfnShape{T, D, F, Do}, dtype, 0)) return NMRF_EINVAL;
     const int bk = dtype == NMRF_F32 ? 32 : 64;
-    int64_t n = T < 1 ? 0 : gemm_floats(T, backward ? D : Do, backward ? 2 * (int64_t)F : F, 1, bk);
-    if (backward && T > 0) {
-        for (int z = 1; z <= 2; ++z) n = std::max(n, gemm_floats(F, D, T, z, bk));
-        n = std::max(n, gemm_floats(Do, F, T, 1, bk));
-        n = std::max(n, colsum_blocks(T) * (2 * (int64_t)F + Do));
-    }
+    int64_t n = 0;
+    if (T > 0 && !backward) n = gemm_floats(T, Do, F, bk);
+    if (T > 0 && backward)
+        n = gemm_floats(T, D, 2 * (int64_t)F, bk) + 2 * gemm_floats(F, D, T, bk) + gemm_floats(Do, F, T, bk) + colsum_blocks(T) * Do +
+            4 * (int64_t)F * gemm_plan(T, F, Do, 1, bk, false, false, 0).tiles_m;
     *floats = n;
     return NMRF_OK;
 }
