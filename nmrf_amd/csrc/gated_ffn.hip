@@ -40,7 +40,7 @@ enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ void act_both(float g, int act, float &value, float &slope) {
     if (act == ACT_SILU) {
-        const float s = 1.0f / (1.0f + exp_of(-g));
+        const float s = __builtin_amdgcn_rcpf(1.0f + exp_of(-g));  // (1 ulp; a division is ten instructions a hidden value)
         value = g == -INFINITY ? 0.f : g * s;
         slope = fmaf(value, 1.0f - s, s);
     } else if (act == ACT_GELU) {
@@ -137,22 +137,38 @@ template <typename T, int ROWS, int BK, bool ALONG, int THREADS> struct Stage {
         if constexpr (ALONG) return c ^ ((i / (16 / CPR)) & (CPR - 1));
         else return c ^ ((2 * ((i & 3) | ((i >> 3) & 1) << 2)) & (CPR - 1));
     }
-    // The operand's tile (rows from m0, contraction from k0).  row_of(i, end): address of (row i of the tile, k0) and of the tensor's end, for
-    // ALONG; base: address of (k0, m0), for ACROSS.  left: values of k from k0 on; rows: rows from m0 on.  A row behind the last is read as
-    // another one (its products are not stored), a value of k behind the last is zero.
-    template <typename RowOf>
-    __device__ __forceinline__ void load(const T *base, int ld, int rows, int left, const T *end, RowOf row_of) {
-        // ACROSS reads over a row's end into the rows behind it (8 of them hold 8 values whatever their width) unless the rows end with a chunk
-        const bool whole = left >= (ALONG || (rows & 7) == 0 ? BK : BK + 8);
+    unsigned off[N];                                               // byte offsets of the chunks from the tile's first value: they do not change with k
+    // ALONG: of_row(i): the matrix row of tile row i (a row behind the last is read as another one: its products are not stored)
+    template <typename OfRow> __device__ __forceinline__ void init(int ld, int rows, OfRow of_row) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int id = threadIdx.x + n * THREADS, i = id / CPR, c = id % CPR * 8;
-            const T *p = ALONG ? row_of(i, end) + c : base + (unsigned)((whole || i < left ? i : 0) * ld) + (c < rows ? c : 0);
+            off[n] = (unsigned)(ALONG ? of_row(i) * ld + c : i * ld + (c < rows ? c : 0)) * (unsigned)sizeof(T);
+        }
+    }
+    // base_of(i): the tile's first value and the end of its tensor (by tile row: two matrices may share a tile); left: values of k from there on
+    template <typename BaseOf>
+    __device__ __forceinline__ void load(int ld, int rows, int left, BaseOf base_of) {
+        // ACROSS reads over a row's end into the rows behind it (8 of them hold 8 values whatever their width) unless the rows end with a chunk
+        if (left >= (ALONG || (rows & 7) == 0 ? BK : BK + 8)) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const T *end, *p = base_of((threadIdx.x + n * THREADS) / CPR, end);
+                const char *q = reinterpret_cast<const char *>(p) + off[n];
+#pragma unroll
+                for (int v = 0; v < V; ++v) __builtin_memcpy(&r[n][v], q + 16 * v, 16);
+            }
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {                              // the last tile: a value of k behind the last is zero
+            const int id = threadIdx.x + n * THREADS, i = id / CPR, c = id % CPR * 8;
+            const T *end, *p = base_of(i, end);
+            p += ALONG ? off[n] / sizeof(T) : (unsigned)((i < left ? i : 0) * ld + (c < rows ? c : 0));
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const T *q = p + v * (8 / V);
-                if (whole) r[n][v] = Vec16<T>::raw(q);
-                else r[n][v] = Vec16<T>::raw_masked(q, ALONG ? max(0, left - c - v * (8 / V)) : (i < left ? 8 : 0), end - q);
+                r[n][v] = Vec16<T>::raw_masked(q, ALONG ? max(0, left - c - v * (8 / V)) : (i < left ? 8 : 0), end - q);
             }
         }
     }
@@ -244,30 +260,19 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
         const int seg = kt / ktiles_seg, k0 = (kt - seg * ktiles_seg) * BK, left = a.K - k0;
         const T *P = static_cast<const T *>(seg ? a.P[1] : a.P[0]);
         const T *Q = static_cast<const T *>(EPI != EPI_DUAL && seg ? a.Q[1] : a.Q[0]);
-        auto none = [](int, const T *&) { return (const T *)nullptr; };
-        if constexpr (PA) {
-            const T *b = P + (int64_t)m0 * a.ldp + k0, *e = P + (int64_t)a.M * a.ldp;
-            sP.load(nullptr, 0, 0, left, e, [&](int i, const T *&) { return b + (unsigned)(min(i, prow - 1) * (int)a.ldp); });
-        } else {
-            sP.load(P + (int64_t)k0 * a.ldp + m0, (int)a.ldp, prow, left, P + (int64_t)a.K * a.ldp, none);
-        }
-        if constexpr (QA) {
-            const T *b = Q + (int64_t)n0 * a.ldq + k0, *e = Q + (int64_t)a.N * a.ldq;
-            if constexpr (EPI == EPI_DUAL) {
-                // of a wave's 16-column tiles the first half are Wg's rows, the second half Wu's
-                const T *b1 = static_cast<const T *>(a.Q[1]) + (int64_t)n0 * a.ldq + k0, *e1 = static_cast<const T *>(a.Q[1]) + (int64_t)a.N * a.ldq;
-                sQ.load(nullptr, 0, 0, left, e, [&](int i, const T *&end) {
-                    const int w = i / (TN * 16), j = i / 16 % TN, n = w * (TN * 8) + j % (TN / 2) * 16 + i % 16;
-                    end = j < TN / 2 ? e : e1;
-                    return (j < TN / 2 ? b : b1) + (unsigned)(min(n, qrow - 1) * (int)a.ldq);
-                });
-            } else {
-                sQ.load(nullptr, 0, 0, left, e, [&](int i, const T *&) { return b + (unsigned)(min(i, qrow - 1) * (int)a.ldq); });
-            }
-        } else {
-            sQ.load(Q + (int64_t)k0 * a.ldq + n0, (int)a.ldq, qrow, left, Q + (int64_t)a.K * a.ldq, none);
-        }
+        const T *pb = P + (PA ? (int64_t)m0 * a.ldp + k0 : (int64_t)k0 * a.ldp + m0), *pe = P + (int64_t)(PA ? a.M : a.K) * a.ldp;
+        sP.load((int)a.ldp, prow, left, [&](int, const T *&end) { end = pe; return pb; });
+        const int64_t qo = QA ? (int64_t)n0 * a.ldq + k0 : (int64_t)k0 * a.ldq + n0, qn = (int64_t)(QA ? a.N : a.K) * a.ldq;
+        const T *Q1 = static_cast<const T *>(a.Q[1]);
+        sQ.load((int)a.ldq, qrow, left, [&](int i, const T *&end) {
+            const T *q = EPI == EPI_DUAL && i / 16 % TN >= TN / 2 ? Q1 : Q;
+            end = q + qn;
+            return q + qo;
+        });
     };
+    sP.init((int)a.ldp, prow, [&](int i) { return min(i, prow - 1); });
+    // (EPI_DUAL: of a wave's 16-column tiles the first half are Wg's rows, the second half Wu's)
+    sQ.init((int)a.ldq, qrow, [&](int i) { return min(EPI == EPI_DUAL ? i / (TN * 16) * (TN * 8) + i / 16 % (TN / 2) * 16 + i % 16 : i, qrow - 1); });
     if (kt0 < kt1) {
         fetch(kt0);
         sP.put(lds[0], pmul);
@@ -635,8 +640,9 @@ void few_launch(const FewArgs &a, hipStream_t st) {
     else hipLaunchKernelGGL((ffn_few_kernel<T, NW, 4>), g, b, 0, st, a);
 }
 
-// Tiles of 128 x 128 where they fill the chip, of 64 x 64 where they do not (192 of the 256 CUs); a plain product with too few tiles of either
-// size splits its contraction over about two blocks a CU, 4 k tiles each at least, and is joined by a second launch.
+// Tiles of 256 x 256 (8 waves, 16-bit types) where their number fills rounds of the 256 CUs to 80 %, of 128 x 128 where they fill the chip, of
+// 64 x 64 where they do not (192 of the 256 CUs); a plain product with too few tiles of either size splits its contraction over about two blocks
+// a CU, 4 k tiles each at least, and is joined by a second launch.
 struct GemmPlan { int tile, tiles_m, tiles_n, splits; };
 // z: problems in the launch; tile: that of the launch, 0: to be chosen
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bool split, int tile) {
@@ -648,6 +654,10 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bo
         return (int64_t)p.tiles_m * p.tiles_n * z;
     };
     const int64_t kt = (k + bk - 1) / bk;
+    if (!tile && bk == 64 && k >= 512) {
+        const int64_t big = tiles(256);
+        if (big >= 205 && big * 5 >= (big + 255) / 256 * 256 * 4) tile = 256;
+    }
     int64_t n = tiles(tile ? tile : 128);
     if (!tile && n < 192 && !(split && n * (kt / 4) >= 192)) n = tiles(64);
     p.splits = split && n < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(512 / n, kt / 4)) : 1;
@@ -697,7 +707,9 @@ int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
         if (blocks > 0x7fffffff) return NMRF_EINVAL;
         q.blocks = (int)n;
     }
-    if (tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (tile == 256) {
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((ffn_gemm_kernel<T, 256, 256, 2, 4, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(512), 0, st, a);
+    } else if (tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     return nmrf_launch_status();
 }
@@ -705,7 +717,7 @@ int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
 int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int bk) {
     int64_t n = 0;
     for (int z = 1; z <= 3; ++z)
-        for (int tile = 0; tile <= 128; tile += 64) {
+        for (int tile : {0, 64, 128, 256}) {
             const int s = gemm_plan(M, N, k, z, bk, false, true, tile).splits;
             n = std::max(n, s > 1 ? (int64_t)s * M * N : 0);
         }
