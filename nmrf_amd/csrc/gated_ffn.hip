@@ -283,17 +283,35 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
     for (int kt = kt0; kt < kt1; ++kt) {
         if (kt + 1 < kt1) fetch(kt + 1);                           // on its way while this tile is multiplied
         const H *lp = lds[cur], *lq = lds[cur] + PL * BM * BK;
+        if constexpr (PL == 1) {
+            // two fragments of P ahead of the products, Q's next ones half way: the LDS is read under the matrix pipe
+            constexpr int S = BK / 32 * TM;
+            uint4 fq[2][TN], fp[4];
 #pragma unroll
-        for (int kk = 0; kk < BK / 32; ++kk) {
-            uint4 fp[TM], fq[TN];
+            for (int j = 0; j < TN; ++j) fq[0][j] = SQ::frag(lq, (wn * TN + j) * 16, 0);
+            fp[0] = SP::frag(lp, wm * TM * 16, 0);
+            fp[1] = SP::frag(lp, (wm * TM + 1) * 16, 0);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fp[i] = SP::frag(lp, (wm * TM + i) * 16, kk);
+            for (int s = 0; s < S; ++s) {
+                const int kk = s / TM, i = s % TM;
+                if (s + 2 < S) fp[(s + 2) & 3] = SP::frag(lp, (wm * TM + (s + 2) % TM) * 16, (s + 2) / TM);
+                if (i == TM / 2 && kk + 1 < BK / 32)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fq[j] = SQ::frag(lq, (wn * TN + j) * 16, kk);
-            if constexpr (PL == 2) {
-                uint4 fl[TN];
+                    for (int j = 0; j < TN; ++j) fq[(kk + 1) & 1][j] = SQ::frag(lq, (wn * TN + j) * 16, kk + 1);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[kk & 1][j], fp[s & 3], acc[i][j], H{});
+            }
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < BK / 32; ++kk) {
+                uint4 fp[TM], fq[TN], fl[TN];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) fp[i] = SP::frag(lp, (wm * TM + i) * 16, kk);
 #pragma unroll
                 for (int j = 0; j < TN; ++j) fl[j] = SQ::frag(lq + SQ::PLANE, (wn * TN + j) * 16, kk);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fq[j] = SQ::frag(lq, (wn * TN + j) * 16, kk);
+                // the small products first: lo hi, hi lo, hi hi
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -304,11 +322,11 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
 #pragma unroll
                     for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[j], pl, acc[i][j], H{});
                 }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[j], fp[i], acc[i][j], H{});
             }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mma(fq[j], fp[i], acc[i][j], H{});
         }
         if (kt + 1 < kt1) {
             sP.put(lds[cur ^ 1], pmul);
@@ -351,9 +369,22 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
             for (int k = 0; k < 4; ++k) v[k] = k < left ? (float)p[k] : 0.f;
         }
     };
-    constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN;
+    constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN, GM = EPI == EPI_DH ? TM : 1;
+    // EPI_DH: g and u of a tile that lies inside, a column tile ahead of their use (loads between the stores would each be waited for)
+    const bool inside = EPI == EPI_DH && m0 + BM <= a.M && n0 + BN <= a.N;
+    uint4 gw[2][GM], uw[2][GM];
+    auto ask = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < GM; ++i) {
+            const int64_t at = (int64_t)(m0 + (wm * TM + i) * 16 + (lane & 15)) * a.ldc + n0 + (wn * JN + j) * 16 + 4 * (lane >> 4);
+            gw[j & 1][i] = Vec16<float>::raw(a.g + at);
+            uw[j & 1][i] = Vec16<float>::raw(a.u + at);
+        }
+    };
+    if (EPI == EPI_DH && inside) ask(0);
 #pragma unroll
     for (int j = 0; j < JN; ++j) {
+        if (EPI == EPI_DH && inside && j + 1 < JN) ask(j + 1);
         const int n = n0 + (wn * JN + j) * 16 + 4 * (lane >> 4), left = a.N - n;
         float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -391,8 +422,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
                 put4(a.C, at, left, v);
             } else if constexpr (EPI == EPI_DH) {
                 float g[4], u[4];
-                getf(static_cast<const float *>(a.g) + at, left, g);
-                getf(static_cast<const float *>(a.u) + at, left, u);
+                if (inside) {
+                    Vec16<float>::unpack(gw[j & 1][i], g);
+                    Vec16<float>::unpack(uw[j & 1][i], u);
+                } else {
+                    getf(a.g + at, left, g);
+                    getf(a.u + at, left, u);
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float value, slope;
@@ -451,12 +487,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
     }
 }
 
-// partial results [splits][n] -> the results (the first one plus a bias of `cols` values), several in one launch: a block owns 256 values; its 4
-// row lanes add the splits l, l + 4, ... in ascending order and the lane sums in ascending order
+// partial results [splits][n] -> the results (the first one plus a bias of `cols` values), several in one launch: a block owns 32 values; its 32
+// row lanes add the splits l, l + 32, ... and 32 threads the lane sums, in a fixed order (bias sums have a partial for every 32 or 64 rows of
+// tokens and few columns: long chains want many lanes)
 struct JoinArgs { const float *parts[7]; void *c[7]; int64_t n[7]; int splits[7], blocks[7]; const void *bias; int cols, count; };
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_join_kernel(JoinArgs a) {
-    __shared__ float sh[4][256];
+    __shared__ float sh[32][33];
     int bid = blockIdx.x, which = 0;
     while (which + 1 < a.count && bid >= a.blocks[which]) bid -= a.blocks[which++];
     const int64_t n = a.n[which];
@@ -464,39 +501,42 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(JoinArgs a) {
     const float *p = a.parts[which];
     T *c = static_cast<T *>(a.c[which]);
     const void *bias = which ? nullptr : a.bias;
-    const int l = threadIdx.x >> 6;
-    for (int64_t i0 = (int64_t)bid * 256; i0 < n; i0 += (int64_t)blocks * 256) {
-        const int64_t i = i0 + (threadIdx.x & 63) * 4;
+    const int l = threadIdx.x >> 3, q4 = (threadIdx.x & 7) * 4;
+    for (int64_t i0 = (int64_t)bid * 32; i0 < n; i0 += (int64_t)blocks * 32) {
+        const int64_t i = i0 + q4;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
         if (i + 4 <= n) {
             int k = l;
-            for (; k + 12 < splits; k += 16) {                   // four loads in flight
+            for (; k + 96 < splits; k += 128) {                    // four loads in flight
                 float v[4][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)(k + 4 * q) * n + i), v[q]);
+                for (int q = 0; q < 4; ++q) Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)(k + 32 * q) * n + i), v[q]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
             }
-            for (; k < splits; k += 4) {
+            for (; k < splits; k += 32) {
                 float v[4];
                 Vec16<float>::unpack(Vec16<float>::raw(p + (int64_t)k * n + i), v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += v[e];
             }
         } else {
-            for (int k = l; k < splits; k += 4)
+            for (int k = l; k < splits; k += 32)
                 for (int e = 0; e < 4; ++e)
                     if (i + e < n) s[e] += p[(int64_t)k * n + i + e];
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh[l][(threadIdx.x & 63) * 4 + e] = s[e];
+        for (int e = 0; e < 4; ++e) sh[l][q4 + e] = s[e];
         __syncthreads();
         const int64_t j = i0 + threadIdx.x;
-        if (j < n) {
-            float v = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
-            if (bias) v += (float)static_cast<const T *>(bias)[j % a.cols];
-            c[j] = (T)v;
+        if (threadIdx.x < 32 && j < n) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k & 3] += sh[k][threadIdx.x];
+            float o = (v[0] + v[1]) + (v[2] + v[3]);
+            if (bias) o += (float)static_cast<const T *>(bias)[j % a.cols];
+            c[j] = (T)o;
         }
     }
 }
@@ -640,25 +680,31 @@ void few_launch(const FewArgs &a, hipStream_t st) {
     else hipLaunchKernelGGL((ffn_few_kernel<T, NW, 4>), g, b, 0, st, a);
 }
 
-// Tiles of 256 x 256 (8 waves, 16-bit types) where their number fills rounds of the 256 CUs to 80 %, of 128 x 128 where they fill the chip, of
-// 64 x 64 where they do not (192 of the 256 CUs); a plain product with too few tiles of either size splits its contraction over about two blocks
-// a CU, 4 k tiles each at least, and is joined by a second launch.
+// The tile of a launch.  fp32 with a short contraction (k <= 256): 64 x 64 -- loads, the split into halves and the epilogue outweigh the products,
+// and five waves a SIMD cover each other where two do not (T = 29 952, D = 128: both projections 106 -> 102 us, dg and du 109 -> 90 us).
+// 16-bit types with k >= 512: 256 x 256 (8 waves) where its rounds of 256 blocks cost less than those of 512 blocks of 128 x 128, a product of
+// the large tile taking 0.77 (operand across: dx 505 -> 389 us at T = 8 192, D = 2 048, F = 5 504) to 0.86 of the time (weight gradients:
+// 841 -> 868 us at three rounds for five) -- but not for dg and du, whose epilogue the one block a CU cannot hide (504 -> 576 us).  Else 128 x 128 where it fills the chip, 64 x 64 where it does not (192 of the 256 CUs).  A plain
+// product with too few tiles splits its contraction over about two blocks a CU, 4 k tiles each at least, and is joined by a second launch.
 struct GemmPlan { int tile, tiles_m, tiles_n, splits; };
+enum { PLAN_PLAIN, PLAN_DUAL, PLAN_DH };
 // z: problems in the launch; tile: that of the launch, 0: to be chosen
-GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, bool dual, bool split, int tile) {
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t k, int z, int bk, int what, int tile) {
     GemmPlan p;
     auto tiles = [&](int t) {
         p.tile = t;
         p.tiles_m = (int)((M + t - 1) / t);
-        p.tiles_n = (int)(dual ? (N + t / 2 - 1) / (t / 2) : (N + t - 1) / t);
+        p.tiles_n = (int)(what == PLAN_DUAL ? (N + t / 2 - 1) / (t / 2) : (N + t - 1) / t);
         return (int64_t)p.tiles_m * p.tiles_n * z;
     };
     const int64_t kt = (k + bk - 1) / bk;
-    if (!tile && bk == 64 && k >= 512) {
-        const int64_t big = tiles(256);
-        if (big >= 205 && big * 5 >= (big + 255) / 256 * 256 * 4) tile = 256;
+    if (!tile && bk == 32 && k <= 256) tile = 64;
+    if (!tile && bk == 64 && k >= 512 && what != PLAN_DH) {
+        const int64_t big = ceil_div64(tiles(256), 256) * 256 * 4, small = ceil_div64(tiles(128), 512) * 512;
+        if (tiles(256) >= 192 && big * 86 < small * 100) tile = 256;
     }
     int64_t n = tiles(tile ? tile : 128);
+    const bool split = what == PLAN_PLAIN;
     if (!tile && n < 192 && !(split && n * (kt / 4) >= 192)) n = tiles(64);
     p.splits = split && n < 192 ? (int)std::max<int64_t>(1, std::min<int64_t>(512 / n, kt / 4)) : 1;
     return p;
@@ -676,7 +722,7 @@ struct Pending {
         j.c[k] = c;
         j.n[k] = n;
         j.splits[k] = splits;
-        j.blocks[k] = (int)std::min<int64_t>(ceil_div64(n, 256), 4096);
+        j.blocks[k] = (int)std::min<int64_t>(ceil_div64(n, 32), 8192);
         ws += (int64_t)splits * n;
         return at;
     }
@@ -696,7 +742,7 @@ int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
     int64_t blocks = 0;
     for (int i = 0; i < a.count; ++i) {
         Problem &q = a.p[i];
-        const GemmPlan p = gemm_plan(q.M, q.N, (int64_t)q.K * q.segs, a.count, BK, EPI == EPI_DUAL, EPI == EPI_PLAIN, tile);
+        const GemmPlan p = gemm_plan(q.M, q.N, (int64_t)q.K * q.segs, a.count, BK, EPI == EPI_DUAL ? PLAN_DUAL : EPI == EPI_DH ? PLAN_DH : PLAN_PLAIN, tile);
         tile = p.tile;                                             // (problems of one launch share the first one's tile)
         q.tiles_m = p.tiles_m;
         q.tiles_n = p.tiles_n;
@@ -708,7 +754,7 @@ int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
         q.blocks = (int)n;
     }
     if (tile == 256) {
-        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((ffn_gemm_kernel<T, 256, 256, 2, 4, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(512), 0, st, a);
+        if constexpr (sizeof(T) == 2 && EPI != EPI_DH) hipLaunchKernelGGL((ffn_gemm_kernel<T, 256, 256, 2, 4, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(512), 0, st, a);
     } else if (tile == 128) hipLaunchKernelGGL((ffn_gemm_kernel<T, 128, 128, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     return nmrf_launch_status();
@@ -718,7 +764,7 @@ int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int bk) {
     int64_t n = 0;
     for (int z = 1; z <= 3; ++z)
         for (int tile : {0, 64, 128, 256}) {
-            const int s = gemm_plan(M, N, k, z, bk, false, true, tile).splits;
+            const int s = gemm_plan(M, N, k, z, bk, PLAN_PLAIN, tile).splits;
             n = std::max(n, s > 1 ? (int64_t)s * M * N : 0);
         }
     return n;
@@ -790,7 +836,7 @@ int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *w
     p.P[0] = dy; p.Q[0] = wd; p.ldp = s.Do; p.ldq = s.F; p.ldc = s.F;
     p.M = (int)s.T; p.N = s.F; p.K = s.Do; p.segs = 1;
     p.C = dg; p.C2 = du; p.g = g; p.u = u; p.slot_p = SLOT_DY; p.slot_q = SLOT_WD; p.slot_out = SLOT_DG;
-    const int sums = 2 * gemm_plan(s.T, s.F, s.Do, 1, BK, false, false, 0).tiles_m;
+    const int sums = 2 * gemm_plan(s.T, s.F, s.Do, 1, BK, PLAN_DH, 0).tiles_m;
     if (dbg) p.sum1 = wait.add(s.F, sums, dbg);
     if (dbu) p.sum2 = wait.add(s.F, sums, dbu);
     if ((rc = gemm_launch<T, true, false, EPI_DH>(a, wait, st)) != NMRF_OK) return rc;
@@ -833,7 +879,7 @@ extern "C" int nmrf_gated_ffn_size(int64_t T, int D, int F, int Do, int dtype, i
     if (T > 0 && !backward) n = gemm_floats(T, Do, F, bk);
     if (T > 0 && backward)
         n = gemm_floats(T, D, 2 * (int64_t)F, bk) + 2 * gemm_floats(F, D, T, bk) + gemm_floats(Do, F, T, bk) + colsum_blocks(T) * Do +
-            4 * (int64_t)F * gemm_plan(T, F, Do, 1, bk, false, false, 0).tiles_m;
+            4 * (int64_t)F * gemm_plan(T, F, Do, 1, bk, PLAN_DH, 0).tiles_m;
     *floats = n;
     return NMRF_OK;
 }

@@ -1,10 +1,11 @@
-"""`ops.modules.MSDeformAttn` (ops/modules/ms_deform_attn.py:28-130) on the HIP operator."""
+"""`ops.modules.MSDeformAttn` (ops/modules/ms_deform_attn.py:28-130) on the HIP operator, and the modules of a training block on theirs."""
 import math
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .blocks import gated_ffn, residual_norm
 from .functions import MSDeformAttnFunction
 
 
@@ -63,3 +64,35 @@ class MSDeformAttn(nn.Module):
         out = MSDeformAttnFunction.apply(value.contiguous(), input_spatial_shapes, input_level_start_index,
                                          loc.contiguous(), aw.contiguous(), self.im2col_step)
         return self.output_proj(out)
+
+
+class GatedFeedForward(nn.Module):
+    """y = down(act(gate(x)) * up(x)) on nmrf_amd.ops.gated_ffn: the gated form of the reference's Mlp (fc2(gelu(fc1 x)), nmrf/models/NMP.py:337, 537,
+    675).  Parameters: gate, up [hidden, dim], down [out, hidden] (nn.Linear's layout and initialisation)."""
+
+    def __init__(self, dim, hidden, out=None, act="silu", bias=True):
+        super().__init__()
+        self.act = act
+        self.gate, self.up, self.down = nn.Linear(dim, hidden, bias), nn.Linear(dim, hidden, bias), nn.Linear(hidden, out or dim, bias)
+
+    def forward(self, x):
+        return gated_ffn(x, self.gate.weight, self.up.weight, self.down.weight, self.gate.bias, self.up.bias, self.down.bias, self.act)
+
+
+class ResidualNorm(nn.Module):
+    """(x, y) -> (out, h) on nmrf_amd.ops.residual_norm: out = x + scale * act(gate) * [post](y), h = next(out) -- the tail of a block and the norm in
+    front of the next one (nmrf/models/NMP.py:337-364).  post: normalise the branch too.  layer_scale: a learned scale for each channel that
+    begins at this value (None: none).  A gate is given with the call."""
+
+    def __init__(self, dim, kind="layer", post=False, layer_scale=None, eps=1e-5, gate_act=None):
+        super().__init__()
+        self.kind, self.eps, self.gate_act, self.post = kind, eps, gate_act, post
+        one = lambda v: nn.Parameter(torch.full((dim,), float(v)))  # noqa: E731
+        self.weight, self.bias = one(1), (one(0) if kind == "layer" else None)
+        if post:
+            self.post_weight, self.post_bias = one(1), (one(0) if kind == "layer" else None)
+        self.layer_scale = None if layer_scale is None else one(layer_scale)
+
+    def forward(self, x, y, gate=None):
+        return residual_norm(x, y, (self.weight, self.bias), (self.post_weight, self.post_bias) if self.post else None, gate, self.gate_act,
+                             self.layer_scale, self.kind, self.eps)
