@@ -67,6 +67,11 @@ __device__ __forceinline__ float act_value(float g, int act) {
 
 // ---- largest magnitudes (fp32 operands): per tensor 256 slots, of which a product takes the maximum --------------------------------------
 enum { SLOT_X = 0, SLOT_WG = 1, SLOT_WU = 2, SLOT_WD = 3, SLOT_H = 4, SLOT_DY = 5, SLOT_DG = 6 };
+// (values that are not finite do not count: they spoil their own row whatever the scale, and must not take the others' bits)
+__device__ __forceinline__ float magnitude(float v) {
+    v = fabsf(v);
+    return v < INFINITY ? v : 0.f;
+}
 struct AbsmaxArgs { const float *p[5]; int64_t n[5]; int slot[5]; unsigned *out; };      // p null: clear the slot (a later kernel fills it)
 __global__ __launch_bounds__(256) void ffn_absmax_kernel(AbsmaxArgs a) {
     __shared__ float sh[4];
@@ -82,21 +87,21 @@ __global__ __launch_bounds__(256) void ffn_absmax_kernel(AbsmaxArgs a) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], fabsf(v[u][k]));
+            for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], magnitude(v[u][k]));
     }
     for (; i < i1; i += 1024)
-        for (int k = 0; k < 4 && i + k < i1; ++k) m[k] = fmaxf(m[k], fabsf(p[i + k]));
+        for (int k = 0; k < 4 && i + k < i1; ++k) m[k] = fmaxf(m[k], magnitude(p[i + k]));
     float x = wave_max(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
     __syncthreads();
     if (threadIdx.x == 0) a.out[a.slot[which] * 256 + blockIdx.x] = __float_as_uint(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
 }
-// power of two that puts the largest magnitude at [2^13, 2^14); 1 for zero, infinity and NaN
+// the power of two that puts the largest magnitude at [2^13, 2^14), 0 where all are zero
 __device__ __forceinline__ int slot_shift(const unsigned *amax, int slot, int count) {
     float m = 0.f;
     for (int i = threadIdx.x & 63; i < 256 * count; i += 64) m = fmaxf(m, __uint_as_float(amax[slot * 256 + i]));
     m = wave_max(m);
-    if (!(m > 0.f) || !(m < INFINITY)) return 0;
+    if (!(m > 0.f)) return 0;
     const int e = (int)((__float_as_uint(m) >> 23) & 0xffu) - 127, sh = 13 - (e < -100 ? -100 : e);
     return __builtin_amdgcn_readfirstlane(sh);
 }
@@ -417,7 +422,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     v[k] = act_value(v[k], args.act) * w[k];
-                    if (k < left) top = fmaxf(top, fabsf(v[k]));
+                    if (PL == 2 && k < left) top = fmaxf(top, magnitude(v[k]));
                 }
                 put4(a.C, at, left, v);
             } else if constexpr (EPI == EPI_DH) {
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
                     act_both(g[k], args.act, value, slope);
                     w[k] = v[k] * value;
                     v[k] = v[k] * u[k] * slope;
-                    if (k < left) top = fmaxf(top, fmaxf(fabsf(v[k]), fabsf(w[k])));
+                    if (PL == 2 && k < left) top = fmaxf(top, fmaxf(magnitude(v[k]), magnitude(w[k])));
                 }
                 put4(a.C, at, left, v);
                 put4(a.C2, at, left, w);
@@ -759,13 +764,14 @@ int gemm_launch(GemmArgs &a, Pending &wait, hipStream_t st) {
     else hipLaunchKernelGGL((ffn_gemm_kernel<T, 64, 64, 2, 2, BK, PA, QA, EPI>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     return nmrf_launch_status();
 }
-// floats a plain product keeps in the workspace, at most (whatever shares its launch)
-int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int bk) {
+// floats a plain product keeps in the workspace: alone in its launch, or at most, whatever shares it
+int64_t gemm_floats(int64_t M, int64_t N, int64_t k, int bk, bool alone) {
     int64_t n = 0;
-    for (int z = 1; z <= 3; ++z)
+    for (int z = 1; z <= (alone ? 1 : 3); ++z)
         for (int tile : {0, 64, 128, 256}) {
             const int s = gemm_plan(M, N, k, z, bk, PLAN_PLAIN, tile).splits;
             n = std::max(n, s > 1 ? (int64_t)s * M * N : 0);
+            if (alone) return n;
         }
     return n;
 }
@@ -876,9 +882,9 @@ extern "C" int nmrf_gated_ffn_size(int64_t T, int D, int F, int Do, int dtype, i
     if (ffn_bad(FfnShape{T, D, F, Do}, dtype, 0)) return NMRF_EINVAL;
     const int bk = dtype == NMRF_F32 ? 32 : 64;
     int64_t n = 0;
-    if (T > 0 && !backward) n = gemm_floats(T, Do, F, bk);
+    if (T > 0 && !backward) n = gemm_floats(T, Do, F, bk, true);
     if (T > 0 && backward)
-        n = gemm_floats(T, D, 2 * (int64_t)F, bk) + 2 * gemm_floats(F, D, T, bk) + gemm_floats(Do, F, T, bk) + colsum_blocks(T) * Do +
+        n = gemm_floats(T, D, 2 * (int64_t)F, bk, true) + 2 * gemm_floats(F, D, T, bk, false) + gemm_floats(Do, F, T, bk, false) + colsum_blocks(T) * Do +
             4 * (int64_t)F * gemm_plan(T, F, Do, 1, bk, PLAN_DH, 0).tiles_m;
     *floats = n;
     return NMRF_OK;

@@ -1555,9 +1555,8 @@ def residual_norm_backward(x, y, gate, scale, post_w, post_b, next_w, next_b, d_
         for i in (4, 5):
             if grads[i] is not None:
                 grads[i].zero_()
-    size = ctypes.c_int64()
-    _lib.check(_lib.load().nmrf_residual_norm_bwd_size(s.t, s.c, s.gate_rows if gate is not None else s.t, ctypes.byref(size)), "residual_norm_bwd")
-    ws = torch.empty(size.value, device=x.device, dtype=torch.float32)
+    # (nmrf_residual_norm_bwd_size: 512 blocks of five parameter rows, and a row for each gate group or block)
+    ws = torch.empty((2560 + max(512, s.t // s.gate_rows if gate is not None else 1)) * s.c, device=x.device, dtype=torch.float32)
     dg, dsc, dpw, dpb, dnw, dnb = (_p(g) for g in grads)
     if d_h is None:
         dnw = dnb = None

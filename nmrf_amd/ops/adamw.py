@@ -71,7 +71,8 @@ class AdamWPlan:
         self._tables = [np.fromiter(map(_data_ptr, x), np.uint64, n) for x in self._lists]
         if len(set(self._tables[0][self._numel > 0].tolist())) != int(np.sum(self._numel > 0)):
             raise NmrfHipError("AdamWPlan: a parameter is in the list twice")
-        self._held = [list(map(torch.Tensor.detach, x)) for x in self._lists]      # (the storage stays even if a tensor's .data is replaced)
+        # (a parameter's address is checked each step; the moments' storage is held, whatever becomes of the tensors)
+        self._held = [list(map(torch.Tensor.detach, x)) for x in self._lists[1:]]
         self._g = np.zeros(n, np.uint64)
         self._hyper = np.zeros((n, 4), np.float32)
         self._betas = np.zeros(4, np.float32)

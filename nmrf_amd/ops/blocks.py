@@ -37,6 +37,11 @@ def refuse_captured_backward(name):
         raise NmrfHipError("%s: a backward pass is not captured into a graph (capture the forward pass, or run it eagerly)" % name)
 
 
+def differentiated(*tensors):
+    """Whether a backward pass may follow (a Function does not see that gradients are switched off)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, post_w, post_b, next_w, next_b, spec):
@@ -117,7 +122,11 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
     s.post, s.next = int(post_norm is not None), int(next_norm is not None)
     x, y = x.contiguous(), y.contiguous()
     gate = None if gate is None else gate.contiguous()
-    return ResidualNormFn.apply(x, y, gate, vec, post_w, post_b, next_w, next_b, s)
+    args = (x, y, gate, vec, post_w, post_b, next_w, next_b)
+    if differentiated(*args):
+        return ResidualNormFn.apply(*args, s)
+    out, h = K.residual_norm(*args, s)
+    return (out, h) if s.next else out
 
 
 _FFN_ACTS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -126,11 +135,9 @@ _FFN_ACTS = {"silu": 0, "gelu": 1, "relu": 2}
 class GatedFfnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        keep = any(ctx.needs_input_grad)
-        y, h, g, u, amax = K.gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep)
-        if keep:
-            ctx.save_for_backward(x, w_gate, w_up, w_down, h, g, u, amax)
-            ctx.act = act
+        y, h, g, u, amax = K.gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, h, g, u, amax)
+        ctx.act = act
         return y
 
     @staticmethod
@@ -165,5 +172,6 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act=
     rows = x.numel() // d
     if rows > 0x7fffffff - 256:
         raise ValueError("gated_ffn: %d rows" % rows)
-    args = [None if t is None else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
-    return GatedFfnFn.apply(x.reshape(rows, d).contiguous(), *args, _FFN_ACTS[act]).view(*x.shape[:-1], do)
+    args = [None if t is None else t.contiguous() for t in (x.reshape(rows, d), w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    y = GatedFfnFn.apply(*args, _FFN_ACTS[act]) if differentiated(*args) else K.gated_ffn(*args, _FFN_ACTS[act], False)[0]
+    return y.view(*x.shape[:-1], do)

@@ -48,17 +48,22 @@ class AdamW(torch.optim.Optimizer):
             return adamw_moment(s["exp_avg"], s["exp_avg_scale"]), adamw_moment(s["exp_avg_sq"], s["exp_avg_sq_scale"], squared=True)
         return s["exp_avg"], s["exp_avg_sq"]
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "min_8bit_size": self.min_8bit_size, "seed": self.seed}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.grad_norm, self._plans = None, {}
+
     def _plan(self, key, items):
         """The plan of the parameters in items, kept while they and their state tensors are the same objects."""
         tensors = [t for p, s, _ in items for t in ((p, s["exp_avg"], s["exp_avg_sq"]) if key[2] == 32 else (
             p, s["exp_avg"], s["exp_avg_sq"], s["exp_avg_scale"], s["exp_avg_sq_scale"]))]
         had = self._plans.get(key)
         if had is not None and len(had[0]) == len(tensors) and all(map(operator.is_, had[0], tensors)) and had[1].unmoved():
-            return had[1]
+            return had
         step = 3 if key[2] == 32 else 5
-        plan = AdamWPlan(*(tensors[i::step] for i in range(step)))
-        self._plans[key] = (tensors, plan)
-        return plan
+        return tensors, AdamWPlan(*(tensors[i::step] for i in range(step)))
 
     @torch.no_grad()
     def step(self, closure=None, max_norm=None):
@@ -84,8 +89,9 @@ class AdamW(torch.optim.Optimizer):
         if len({k[0] for k in sets}) > 1 and max_norm is not None:
             raise NotImplementedError("AdamW: clipping over parameters on several devices")
         plans = []
+        self._plans = {key: self._plan(key, items) for key, items in sets.items()}
         for key, items in sets.items():
-            plan = self._plan(key, items)
+            plan = self._plans[key][1]
             with torch.cuda.device(key[0]):
                 plan.bind([p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _, _ in items])
             plans.append((plan, key, items))

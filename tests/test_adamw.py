@@ -89,6 +89,13 @@ def test_state_dict_is_torchs_and_other_bits_are_refused():
         O.AdamW(p).load_state_dict(t.state_dict())
 
 
+def test_optimizer_is_copied_with_its_settings():
+    import copy
+    o = O.AdamW([torch.nn.Parameter(torch.zeros(4))], lr=0.5, state_bits=8, min_8bit_size=7, seed=3)
+    c = copy.deepcopy(o)
+    assert (c.state_bits, c.min_8bit_size, c.seed, c.param_groups[0]["lr"]) == (8, 7, 3, 0.5) and c.step() is None
+
+
 # ---- the formula ----------------------------------------------------------------------------------------------------------------------
 def _case(sizes, dtype, bits, seed, odd=False):
     """Parameters, gradients and moments as views of storage with sentinels between them (odd: none of them aligned to 16 bytes)."""
@@ -469,6 +476,11 @@ def test_optimizer_sees_new_storage_and_mixed_types():
     # constant gradients: m / sqrt(v) = 1 after the bias corrections, two steps of 0.1 (8 bits: codes within 2^-4 and 2^-5 of the moments)
     assert abs(float(a[0][0]) - 0.8) < 1e-5 and abs(float(a[1][0]) - 0.8) <= 0.1 * (2 ** -4 + 2 ** -5) * 1.5 + 0.8 * 2 ** -8
     assert abs(float(o.grad_norm) - math.sqrt(9500)) < 1e-3
+    for b in (0.91, 0.92, 0.93):                                    # a schedule that moves the betas: no plan is kept for the old ones
+        o.param_groups[0]["betas"] = (b, 0.999)
+        o.step()
+    assert len(o._plans) == 2
+    o.state[a[0]]["step"] = o.state[a[1]]["step"] = 2
     a[0].grad = torch.ones(500, device="cuda")[:, None].expand(500, 1)[:, 0]
     a[1].grad = None
     o.step()

@@ -158,6 +158,26 @@ def test_few_tokens(t, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_tiles(dtype):
+    """Enough tiles of 256 x 256 to be chosen, none of them whole at the edges; weight gradients with and without a split contraction."""
+    v, dy = case(4099, 520, 1600, 515, dtype, True, seed=21)
+    check(v, dy, "silu")
+
+
+@pytest.mark.gpu
+def test_no_gradient_mode_takes_the_short_way():
+    """Parameters that require gradients under no_grad: the same call as without them, bit for bit (one token: the weights are streamed)."""
+    for t in (1, 200):
+        v, dy = case(t, 64, 96, 48, torch.bfloat16, True, seed=22)
+        want, _ = run(v, dy, "silu", grad=False)
+        leaves = {k: x.clone().requires_grad_(True) for k, x in v.items()}
+        with torch.no_grad():
+            y = gated_ffn(*[leaves[k] for k in NAMES])
+        assert torch.equal(y, want) and not y.requires_grad
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 def test_leading_dimensions_and_shared_rows(act):
     v, dy = case(0, 64, 96, 80, torch.float32, True, seed=3, lead=(2, 3, 35))
@@ -198,6 +218,12 @@ def test_values_that_are_not_finite_stay_in_their_row(dtype):
     keep = torch.ones(200, dtype=torch.bool, device="cuda")
     keep[[7, 150]] = False
     assert bool(torch.isfinite(y[keep]).all()) and bool(torch.isnan(y[7]).all()) and not bool(torch.isfinite(y[150]).any())
+    if dtype == torch.float32:                                      # a row that is not finite leaves the scale to the others, large or small
+        for c in (1e7, 1e-7):
+            w = {**v, "x": v["x"] * c, "w_gate": v["w_gate"] / c, "w_up": v["w_up"] / c}
+            other, _ = run(w, dy, "silu", grad=False)
+            want, _ = formula({**w, "x": torch.where(keep[:, None], w["x"], torch.zeros_like(w["x"]))}, dy, "silu")
+            assert float((other[keep].double() - want["y"][0][keep]).abs().max()) <= 6 * (math.sqrt(160) + 16 + 8) * W * float(want["y"][1].max())
     few, _ = run({**v, "x": v["x"][:20]}, dy[:20], "silu", grad=False)
     assert bool(torch.isnan(few[7]).all()) and bool(torch.isfinite(few[[i for i in range(20) if i != 7]]).all())
 
