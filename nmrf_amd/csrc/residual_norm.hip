@@ -71,9 +71,14 @@ template <int LPR> struct RowSum {
         }
     }
     __device__ __forceinline__ float one(float a) {
-        float b = 0.f;
         if constexpr (LPR <= 64) return lanes_sum<LPR>(a);
-        two(a, b);
+        a = wave_sum_nolds(a);
+        if ((threadIdx.x & 63) == 0) sh[turn][0][threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = 0.f;
+#pragma unroll
+        for (int w = 0; w < LPR / 64; ++w) a += sh[turn][0][w];
+        turn ^= 1;
         return a;
     }
 };
@@ -190,9 +195,14 @@ template <typename T, int LPR, int E, int FIT> struct Row {
             su += u[e];
             sx = fmaf(u[e], vhat[e], sx);
         }
-        rs.two(su, sx);
-        su = rms ? 0.f : su / C;
-        sx = sx / C;
+        if (rms) {
+            sx = rs.one(sx);
+            su = 0.f;
+        } else {
+            rs.two(su, sx);
+        }
+        su *= 1.0f / C;
+        sx *= 1.0f / C;
 #pragma unroll
         for (int e = 0; e < K; ++e) u[e] = rstd * (u[e] - su - vhat[e] * sx);
     }
@@ -537,11 +547,12 @@ int rn_gate_mode(const void *gate, int64_t T, int C, int64_t R, int cols) {
     if (cols == C && C > 1) return R == 1 ? GATE_ELEM : GATE_GROUP;
     return R == 1 ? GATE_ROW : GATE_GROUP_ONE;
 }
-// the backward grid: items of rows of one gate group each, about 512 blocks (2 per CU: more partial rows cost more than they hide)
+// the backward grid: items of rows of one gate group each, about 512 blocks (2 per CU; rows of 8 waves: one per CU,
+// which is what their registers leave room for: more partial rows cost more than they hide)
 struct RnPlan { int64_t items, chunks, rows; int blocks; };
 RnPlan rn_plan(int64_t T, int64_t span, int lpr) {
     const int side = lpr <= 256 ? 256 / lpr : 1;                   // rows a block works on at once
-    const int64_t target = 512, groups = T / span;
+    const int64_t target = lpr == 512 ? 256 : 512, groups = T / span;
     RnPlan p;
     int64_t chunks = groups >= target ? 1 : target / groups;
     const int64_t most = ceil_div64(span, side);

@@ -2,6 +2,7 @@
 pointers and the CURRENT torch stream.  PyTorch is plumbing here (memory + streams); all arithmetic
 of these ops happens in libnmrf_hip.so.  Every wrapper refuses non-CUDA tensors: there is no
 fallback path."""
+import collections
 import ctypes
 import functools
 import os
@@ -1530,40 +1531,37 @@ def adamw_moment(code, scale, squared=False):
     return out
 
 
-# the norms around a block (csrc/residual_norm.hip).  `spec`: the call's numbers as nmrf_amd.ops.residual_norm has checked them
-class ResidualNormSpec:
-    __slots__ = ("t", "c", "kind", "eps", "gate_rows", "gate_cols", "gate_act", "scale_value", "post", "next", "params_f32")
+# the norms around a block (csrc/residual_norm.hip): the call's numbers as nmrf_amd.ops.residual_norm has checked them
+ResidualNormSpec = collections.namedtuple("ResidualNormSpec", "t c kind eps gate_rows gate_cols gate_act scale_value post next params_f32 dtype")
 
 
 @_on_device
 def residual_norm(x, y, gate, scale, post_w, post_b, next_w, next_b, s):
-    out, h = torch.empty_like(x), (torch.empty_like(x) if s.next else None)
-    _lib.check(_lib.load().nmrf_residual_norm(_p(x), _p(y), s.t, s.c, DTYPE_CODE[x.dtype], s.kind, s.eps, _p(gate), s.gate_rows, s.gate_cols,
-                                              s.gate_act, s.scale_value, _p(scale), s.post, _p(post_w), _p(post_b), _p(next_w), _p(next_b),
-                                              s.params_f32, _p(out), _p(h), _raw_stream()), "residual_norm")
+    t, c, kind, eps, rows, cols, act, value, post, nxt, f32, dtype = s
+    out, h = torch.empty_like(x), (torch.empty_like(x) if nxt else None)
+    _lib.check(_lib.load().nmrf_residual_norm(_p(x), _p(y), t, c, dtype, kind, eps, _p(gate), rows, cols, act, value, _p(scale), post, _p(post_w),
+                                              _p(post_b), _p(next_w), _p(next_b), f32, _p(out), _p(h), _raw_stream()), "residual_norm")
     return out, h
 
 
 @_on_device
 def residual_norm_backward(x, y, gate, scale, post_w, post_b, next_w, next_b, d_out, d_h, s, want):
     """-> gradients of (x, y, gate, scale, post_w, post_b, next_w, next_b); want: which of the last six (None elsewhere)."""
+    t, c, kind, eps, rows, cols, act, value, post, _, f32, dtype = s
     dx, dy = torch.empty_like(x), torch.empty_like(y)
-    grads = [torch.empty_like(t) if t is not None and w else None for t, w in zip((gate, scale, post_w, post_b, next_w, next_b), want)]
-    if s.t == 0:
+    dg, dsc, dpw, dpb, dnw, dnb = grads = [torch.empty_like(p) if w else None for p, w in zip((gate, scale, post_w, post_b, next_w, next_b), want)]
+    if t == 0:
         return [dx, dy] + [None if g is None else g.zero_() for g in grads]
     if d_h is None:                                                    # (h was not used: its norm's parameters have no share)
-        for i in (4, 5):
-            if grads[i] is not None:
-                grads[i].zero_()
-    # (nmrf_residual_norm_bwd_size: 512 blocks of five parameter rows, and a row for each gate group or block)
-    ws = torch.empty((2560 + max(512, s.t // s.gate_rows if gate is not None else 1)) * s.c, device=x.device, dtype=torch.float32)
-    dg, dsc, dpw, dpb, dnw, dnb = (_p(g) for g in grads)
-    if d_h is None:
+        for g in (dnw, dnb):
+            if g is not None:
+                g.zero_()
         dnw = dnb = None
-    _lib.check(_lib.load().nmrf_residual_norm_bwd(_p(x), _p(y), _p(d_out), _p(d_h), s.t, s.c, DTYPE_CODE[x.dtype], s.kind, s.eps, _p(gate),
-                                                  s.gate_rows, s.gate_cols, s.gate_act, s.scale_value, _p(scale), s.post, _p(post_w), _p(post_b),
-                                                  _p(next_w), s.params_f32, _p(dx), _p(dy), dg, dsc, dpw, dpb, dnw, dnb, _p(ws), ws.numel(),
-                                                  _raw_stream()), "residual_norm_bwd")
+    # (nmrf_residual_norm_bwd_size: 512 blocks of five parameter rows, and a row for each gate group or block)
+    ws = torch.empty((2560 + max(512, t // rows if gate is not None else 1)) * c, device=x.device, dtype=torch.float32)
+    _lib.check(_lib.load().nmrf_residual_norm_bwd(_p(x), _p(y), _p(d_out), _p(d_h), t, c, dtype, kind, eps, _p(gate), rows, cols, act, value,
+                                                  _p(scale), post, _p(post_w), _p(post_b), _p(next_w), f32, _p(dx), _p(dy), _p(dg), _p(dsc),
+                                                  _p(dpw), _p(dpb), _p(dnw), _p(dnb), _p(ws), ws.numel(), _raw_stream()), "residual_norm_bwd")
     return [dx, dy] + grads
 
 

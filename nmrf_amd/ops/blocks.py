@@ -11,23 +11,21 @@ from .._lib import NmrfHipError
 _GATE_ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
 
 
-def check_rows(name, **tensors):
-    """One device, one type of fp32 / bf16 / fp16, on the GPU; -> that type."""
-    ref = None
-    for k, t in tensors.items():
+def check_rows(name, names, tensors):
+    """One device, one type of fp32 / bf16 / fp16, on the GPU."""
+    ref = tensors[0]
+    dtype, device = ref.dtype, ref.device
+    if not ref.is_cuda:
+        raise NmrfHipError("%s runs on the MI355X only: %s is a %s tensor (no CPU fallback exists by design)" % (name, names[0], device))
+    if dtype not in K.DTYPE_CODE:
+        raise NmrfHipError("%s: %s is fp32, bf16 or fp16, got %s" % (name, names[0], dtype))
+    for k, t in zip(names, tensors):
         if t is None:
             continue
-        if not t.is_cuda:
-            raise NmrfHipError("%s runs on the MI355X only: %s is a %s tensor (no CPU fallback exists by design)" % (name, k, t.device))
-        if ref is None:
-            ref = t
-            if t.dtype not in K.DTYPE_CODE:
-                raise NmrfHipError("%s: %s is fp32, bf16 or fp16, got %s" % (name, k, t.dtype))
-        if t.device != ref.device:
-            raise NmrfHipError("%s: tensors live on different devices: %s and %s" % (name, ref.device, t.device))
-        if t.dtype != ref.dtype:
-            raise NmrfHipError("%s: %s is %s, expected %s" % (name, k, t.dtype, ref.dtype))
-    return ref.dtype
+        if t.device != device:
+            raise NmrfHipError("%s: tensors live on different devices: %s and %s" % (name, device, t.device))
+        if t.dtype != dtype:
+            raise NmrfHipError("%s: %s is %s, expected %s" % (name, k, t.dtype, dtype))
 
 
 def refuse_captured_backward(name):
@@ -91,38 +89,36 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
         raise ValueError("residual_norm: kind is 'layer' or 'rms', got %r" % (kind,))
     if gate_act not in _GATE_ACTS:
         raise ValueError("residual_norm: gate_act is None, 'sigmoid' or 'tanh', got %r" % (gate_act,))
-    if x.shape != y.shape or x.dim() < 1:
-        raise ValueError("residual_norm: x %s and y %s differ" % (tuple(x.shape), tuple(y.shape)))
+    shape = x.shape
+    if shape != y.shape or not shape:
+        raise ValueError("residual_norm: x %s and y %s differ" % (tuple(shape), tuple(y.shape)))
     if not eps >= 0:
         raise ValueError("residual_norm: eps %r" % (eps,))
-    c = x.shape[-1]
+    c = shape[-1]
     if not 1 <= c <= 8192:
         raise ValueError("residual_norm: %d channels are not in 1 ... 8192" % c)
     post_w, post_b = post_norm if post_norm is not None else (None, None)
     next_w, next_b = next_norm if next_norm is not None else (None, None)
     vec = scale if isinstance(scale, torch.Tensor) else None
-    dtype = check_rows("residual_norm", x=x, y=y, gate=gate)
-    s = K.ResidualNormSpec()
-    s.params_f32 = 0
-    params = dict(scale=vec, post_weight=post_w, post_bias=post_b, next_weight=next_w, next_bias=next_b)
-    have = {k: t for k, t in params.items() if t is not None}
-    for k, t in have.items():
-        if tuple(t.shape) != (c,):
+    check_rows("residual_norm", ("x", "y", "gate"), (x, y, gate))
+    device, of = x.device, None                                         # of: the parameters' type
+    params = (vec, post_w, post_b, next_w, next_b)
+    for k, t in zip(("scale", "post_weight", "post_bias", "next_weight", "next_bias"), params):
+        if t is None:
+            continue
+        if t.shape != (c,):
             raise ValueError("residual_norm: %s has shape %s, expected (%d,)" % (k, tuple(t.shape), c))
-        if t.device != x.device or not t.is_contiguous():
-            raise NmrfHipError("residual_norm: %s is not a contiguous tensor on %s" % (k, x.device))
-    kinds = {t.dtype for t in have.values()}
-    if kinds - {dtype, torch.float32} or len(kinds) > 1:
-        raise NmrfHipError("residual_norm: weights, biases and the scale vector are all %s or all torch.float32, got %s" % (dtype, sorted(map(str, kinds))))
-    s.params_f32 = int(bool(kinds) and kinds == {torch.float32})
-    s.c, s.t = c, x.numel() // c
-    s.gate_rows, s.gate_cols = _gate_layout(x, gate) if gate is not None else (1, 1)
-    s.gate_act, s.kind, s.eps = _GATE_ACTS[gate_act], int(kind == "rms"), float(eps)
-    s.scale_value = 1.0 if scale is None or vec is not None else float(scale)
-    s.post, s.next = int(post_norm is not None), int(next_norm is not None)
-    x, y = x.contiguous(), y.contiguous()
-    gate = None if gate is None else gate.contiguous()
-    args = (x, y, gate, vec, post_w, post_b, next_w, next_b)
+        if t.device != device or not t.is_contiguous():
+            raise NmrfHipError("residual_norm: %s is not a contiguous tensor on %s" % (k, device))
+        if of is None:
+            of = t.dtype
+        if t.dtype != of or (of != x.dtype and of != torch.float32):
+            raise NmrfHipError("residual_norm: weights, biases and the scale vector are all %s or all torch.float32, got %s for %s" % (x.dtype, t.dtype, k))
+    rows, cols = _gate_layout(x, gate) if gate is not None else (1, 1)
+    s = K.ResidualNormSpec(x.numel() // c, c, int(kind == "rms"), float(eps), rows, cols, _GATE_ACTS[gate_act],
+                           1.0 if scale is None or vec is not None else float(scale), int(post_norm is not None), int(next_norm is not None),
+                           int(of == torch.float32), K.DTYPE_CODE[x.dtype])
+    args = (x.contiguous(), y.contiguous(), None if gate is None else gate.contiguous(), *params)
     if differentiated(*args):
         return ResidualNormFn.apply(*args, s)
     out, h = K.residual_norm(*args, s)
@@ -130,6 +126,7 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
 
 
 _FFN_ACTS = {"silu": 0, "gelu": 1, "relu": 2}
+_FFN_NAMES = ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
 
 
 class GatedFfnFn(torch.autograd.Function):
@@ -162,13 +159,12 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act=
         raise ValueError("gated_ffn: x [..., D], w_gate, w_up [F, D], w_down [D', F]; got %s, %s, %s" % (
             tuple(x.shape), tuple(w_gate.shape), tuple(w_down.shape)))
     d, (f, do) = x.shape[-1], (w_gate.shape[0], w_down.shape[0])
-    for name, t, shape in (("w_gate", w_gate, (f, d)), ("w_up", w_up, (f, d)), ("w_down", w_down, (do, f)), ("b_gate", b_gate, (f,)),
-                           ("b_up", b_up, (f,)), ("b_down", b_down, (do,))):
-        if t is not None and tuple(t.shape) != shape:
+    for name, t, shape in zip(_FFN_NAMES[1:], (w_gate, w_up, w_down, b_gate, b_up, b_down), ((f, d), (f, d), (do, f), (f,), (f,), (do,))):
+        if t is not None and t.shape != shape:
             raise ValueError("gated_ffn: %s has shape %s, expected %s" % (name, tuple(t.shape), shape))
     if min(d, f, do) < 1 or max(d, f, do) > 1 << 22:
         raise ValueError("gated_ffn: widths %d, %d, %d are not in 1 ... 2^22" % (d, f, do))
-    check_rows("gated_ffn", x=x, w_gate=w_gate, w_up=w_up, w_down=w_down, b_gate=b_gate, b_up=b_up, b_down=b_down)
+    check_rows("gated_ffn", _FFN_NAMES, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
     rows = x.numel() // d
     if rows > 0x7fffffff - 256:
         raise ValueError("gated_ffn: %d rows" % rows)
