@@ -223,7 +223,7 @@ template <typename T, int ROWS, int BK, bool ALONG, int THREADS> struct Stage {
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int BK, bool PA, bool QA, int EPI>
-__global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm_kernel(GemmArgs args) {
     using H = Half<T>;
     constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, PL = sizeof(T) == 4 ? 2 : 1;
     using SP = Stage<T, BM, BK, PA, THREADS>;
@@ -278,6 +278,22 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
     sP.init((int)a.ldp, prow, [&](int i) { return min(i, prow - 1); });
     // (EPI_DUAL: of a wave's 16-column tiles the first half are Wg's rows, the second half Wu's)
     sQ.init((int)a.ldq, qrow, [&](int i) { return min(EPI == EPI_DUAL ? i / (TN * 16) * (TN * 8) + i / 16 % (TN / 2) * 16 + i % 16 : i, qrow - 1); });
+    constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN, GM = EPI == EPI_DH ? TM : 1, GJ = EPI == EPI_DH ? TN : 1, EARLY = EPI == EPI_DH && TN == 2 ? 2 : 0;
+    // EPI_DH: g and u of a tile that lies inside, all before the first store (a load between stores is waited for by itself): before the contraction
+    // where the registers hold them beside it (64 x 64), else behind it
+    const bool inside = EPI == EPI_DH && m0 + BM <= a.M && n0 + BN <= a.N;
+    uint4 gw[GJ][GM], uw[GJ][GM];
+    auto ask = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < GM; ++i) {
+            const int64_t at = (int64_t)(m0 + (wm * TM + i) * 16 + (lane & 15)) * a.ldc + n0 + (wn * JN + j) * 16 + 4 * (lane >> 4);
+            gw[j][i] = Vec16<float>::raw(a.g + at);
+            uw[j][i] = Vec16<float>::raw(a.u + at);
+        }
+    };
+    if (EARLY && inside)
+#pragma unroll
+        for (int j = 0; j < EARLY; ++j) ask(j);
     if (kt0 < kt1) {
         fetch(kt0);
         sP.put(lds[0], pmul);
@@ -374,22 +390,11 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
             for (int k = 0; k < 4; ++k) v[k] = k < left ? (float)p[k] : 0.f;
         }
     };
-    constexpr int JN = EPI == EPI_DUAL ? TN / 2 : TN, GM = EPI == EPI_DH ? TM : 1;
-    // EPI_DH: g and u of a tile that lies inside, a column tile ahead of their use (loads between the stores would each be waited for)
-    const bool inside = EPI == EPI_DH && m0 + BM <= a.M && n0 + BN <= a.N;
-    uint4 gw[2][GM], uw[2][GM];
-    auto ask = [&](int j) {
+    if (EPI == EPI_DH && inside)
 #pragma unroll
-        for (int i = 0; i < GM; ++i) {
-            const int64_t at = (int64_t)(m0 + (wm * TM + i) * 16 + (lane & 15)) * a.ldc + n0 + (wn * JN + j) * 16 + 4 * (lane >> 4);
-            gw[j & 1][i] = Vec16<float>::raw(a.g + at);
-            uw[j & 1][i] = Vec16<float>::raw(a.u + at);
-        }
-    };
-    if (EPI == EPI_DH && inside) ask(0);
+        for (int j = EARLY; j < JN; ++j) ask(j);
 #pragma unroll
     for (int j = 0; j < JN; ++j) {
-        if (EPI == EPI_DH && inside && j + 1 < JN) ask(j + 1);
         const int n = n0 + (wn * JN + j) * 16 + 4 * (lane >> 4), left = a.N - n;
         float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -428,8 +433,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(GemmArgs args) {
             } else if constexpr (EPI == EPI_DH) {
                 float g[4], u[4];
                 if (inside) {
-                    Vec16<float>::unpack(gw[j & 1][i], g);
-                    Vec16<float>::unpack(uw[j & 1][i], u);
+                    Vec16<float>::unpack(gw[j][i], g);
+                    Vec16<float>::unpack(uw[j][i], u);
                 } else {
                     getf(a.g + at, left, g);
                     getf(a.u + at, left, u);
