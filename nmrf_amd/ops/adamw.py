@@ -96,11 +96,12 @@ class AdamWPlan:
                 raise NmrfHipError("AdamW: a tensor has %d elements, its parameter needs %d" % (t.numel(), n))
 
     def unmoved(self):
-        """Whether every parameter still has the storage the tables name (p.data = ... gives it another)."""
-        return np.array_equal(np.fromiter(map(_data_ptr, self.params), np.uint64, self.n), self._tables[0])
+        """Whether every parameter still has the storage the tables name, and its layout (p.data = ... gives it another)."""
+        return np.array_equal(np.fromiter(map(_data_ptr, self.params), np.uint64, self.n), self._tables[0]) and all(map(_contiguous, self.params))
 
     def bind(self, grads):
-        """Check one step's gradients (parameter order, the parameters' type and sizes) and take their addresses."""
+        """Check one step's gradients (parameter order, the parameters' type and sizes) and take their addresses: the caller keeps them until
+        the update has been launched."""
         if len(grads) != self.n:
             raise ValueError("AdamWPlan: %d gradients for %d parameters" % (len(grads), self.n))
         self._check(grads, self.dtype, self._numel)
@@ -150,7 +151,7 @@ class AdamWPlan:
             with torch.cuda.device(self.device):
                 return self.step(grads, step, lr, betas, eps, max_norm, seed)
         if not self.unmoved():
-            raise NmrfHipError("AdamWPlan: a parameter has new storage: build a new plan")
+            raise NmrfHipError("AdamWPlan: a parameter has new storage or another layout: build a new plan")
         self.bind(grads)
         norm = coef = None
         if max_norm is not None:

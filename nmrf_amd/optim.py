@@ -88,12 +88,14 @@ class AdamW(torch.optim.Optimizer):
             return loss
         if len({k[0] for k in sets}) > 1 and max_norm is not None:
             raise NotImplementedError("AdamW: clipping over parameters on several devices")
-        plans = []
+        plans, held = [], []                                           # held: copies of strided gradients, until the update has been launched
         self._plans = {key: self._plan(key, items) for key, items in sets.items()}
         for key, items in sets.items():
             plan = self._plans[key][1]
             with torch.cuda.device(key[0]):
-                plan.bind([p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _, _ in items])
+                grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _, _ in items]
+                plan.bind(grads)
+            held.append(grads)
             plans.append((plan, key, items))
         coef = None
         if max_norm is not None:

@@ -485,3 +485,35 @@ def test_optimizer_sees_new_storage_and_mixed_types():
     a[1].grad = None
     o.step()
     assert o.state[a[1]]["step"] == 2 and o.state[a[0]]["step"] == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_strided_gradients_of_several_types_step_as_contiguous_ones(bits):
+    """The contiguous copies of strided gradients live until every type's update has been launched (a copy freed early is where the next
+    type's copy, or the norm's partial sums, would go): the same bits as from contiguous gradients."""
+    def run(strided):
+        gen = torch.Generator("cpu").manual_seed(3)
+        params = [torch.nn.Parameter(torch.randn(96, 128, generator=gen).to("cuda", t)) for t in (torch.float32, torch.bfloat16, torch.float16) * 2]
+        o = O.AdamW(params, lr=0.01, state_bits=bits)
+        for _ in range(3):
+            for p in params:
+                g = torch.randn(96, 128, generator=gen).to("cuda", p.dtype)
+                p.grad = g.t().contiguous().t() if strided else g
+            o.step(max_norm=0.5)
+        return [p.detach() for p in params] + [o.grad_norm]
+
+    assert run(True)[0].shape == (96, 128)
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_plan_refuses_a_parameter_whose_layout_changed():
+    p = torch.nn.Parameter(torch.ones(64, 128, device="cuda"))
+    z = lambda: torch.zeros(64, 128, device="cuda")  # noqa: E731
+    plan = AdamWPlan([p], [z()], [z()])
+    plan.step([torch.ones(64, 128, device="cuda")], 1, 0.1)
+    p.data = p.data.t()
+    with pytest.raises(_lib.NmrfHipError, match="layout"):
+        plan.step([torch.ones(128, 64, device="cuda")], 2, 0.1)
