@@ -13,6 +13,11 @@
 //
 // Few tokens (up to 64): the weights are read once and nothing else matters; ffn_few_kernel streams them from memory into the matrix pipe's
 // operand layout without LDS, a block's 8 waves sharing the contraction.
+//
+// Measured (kernel time): bf16, T = 8 192, D = 2 048, F = 5 504: both projections 529 us (369 GFLOP, 698 TFLOP/s), the second matrix 238 us (776),
+// dg and du 474 us (390: 541 MB of g, u, dg and du go through its epilogue), dx 386 us (956), weight gradients 761 us (728).  fp32, T = 29 952,
+// D = 128, F = 512: 102, 40, 90, 68 and 60 us (44 to 198 TFLOP/s of fp32 work, three products each).  One token, bf16, D = 4 096,
+// F = 11 008: 33 + 20 us (270 MB, 5.1 TB/s).
 #include "common.h"
 #include "elem.h"
 #include <algorithm>
@@ -603,7 +608,7 @@ struct FewArgs {
 };
 template <typename T, int NW, int MT>
 __global__ __launch_bounds__(512) void ffn_few_kernel(FewArgs a) {
-    constexpr int V = 16 / sizeof(T), STEP = 4 * V, U = 4;         // values of a lane, k of a step, steps in flight
+    constexpr int V = 16 / sizeof(T), STEP = 4 * V, U = NW * MT == 1 ? 8 : 4;      // values of a lane, k of a step, steps in flight
     __shared__ f32x4 red[8][NW * MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = blockIdx.x * 16;
     const int row = min(n0 + (lane & 15), a.N - 1);
@@ -629,25 +634,34 @@ __global__ __launch_bounds__(512) void ffn_few_kernel(FewArgs a) {
             return mma(p, q, c, T{});
         }
     };
+    // whole steps, U at a time; those behind the last one read it again and count as zeros (a step by itself waits for memory by itself), and 8 in
+    // flight for one matrix and one token tile, which have the registers: second matrix of one token, D = 4 096, F = 11 008, 27 -> 20 us
+    const int whole = min(s1, a.K / STEP);
     int st = s0;
-    for (; st + U <= s1 && (st + U) * STEP <= a.K; st += U) {
+    for (; st < whole; st += U) {
         uint4 wv[U][NW], xv[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = (st + u) * STEP + V * (lane >> 4);
+            const int k = min(st + u, whole - 1) * STEP + V * (lane >> 4);
 #pragma unroll
             for (int s = 0; s < NW; ++s) wv[u][s] = Vec16<T>::raw(w[s] + k);
 #pragma unroll
             for (int t = 0; t < MT; ++t) xv[u][t] = Vec16<T>::raw(x[t] + k);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            const bool on = st + u < whole;
 #pragma unroll
-            for (int s = 0; s < NW; ++s)
+            for (int t = 0; t < MT; ++t) xv[u][t] = on ? xv[u][t] : uint4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < NW; ++s) {
+                wv[u][s] = on ? wv[u][s] : uint4{0, 0, 0, 0};
 #pragma unroll
                 for (int t = 0; t < MT; ++t) acc[s][t] = fma1(wv[u][s], xv[u][t], acc[s][t]);
+            }
+        }
     }
-    for (; st < s1; ++st) {
+    for (st = max(s0, whole); st < s1; ++st) {
         const int k = st * STEP + V * (lane >> 4), left = max(0, min(V, a.K - k)), kk = left ? k : 0;
         uint4 xv[MT];
 #pragma unroll
@@ -693,8 +707,9 @@ void few_launch(const FewArgs &a, hipStream_t st) {
 // The tile of a launch.  fp32 with a short contraction (k <= 256): 64 x 64 -- loads, the split into halves and the epilogue outweigh the products,
 // and five waves a SIMD cover each other where two do not (T = 29 952, D = 128: both projections 106 -> 102 us, dg and du 109 -> 90 us).
 // 16-bit types with k >= 512: 256 x 256 (8 waves) where its rounds of 256 blocks cost less than those of 512 blocks of 128 x 128, a product of
-// the large tile taking 0.77 (operand across: dx 505 -> 389 us at T = 8 192, D = 2 048, F = 5 504) to 0.86 of the time (weight gradients:
-// 841 -> 868 us at three rounds for five) -- but not for dg and du, whose epilogue the one block a CU cannot hide (504 -> 576 us).  Else 128 x 128 where it fills the chip, 64 x 64 where it does not (192 of the 256 CUs).  A plain
+// the large tile taking 0.77 (operand across: dx 505 -> 386 us at T = 8 192, D = 2 048, F = 5 504) to 0.86 of the time (weight gradients:
+// 761 us in five rounds of the small one, 868 in three of the large) -- but not for dg and du, whose epilogue the one block a CU cannot hide
+// (474 us with the small tile, 576 with the large).  Else 128 x 128 where it fills the chip, 64 x 64 where it does not (192 of the 256 CUs).  A plain
 // product with too few tiles splits its contraction over about two blocks a CU, 4 k tiles each at least, and is joined by a second launch.
 struct GemmPlan { int tile, tiles_m, tiles_n, splits; };
 enum { PLAN_PLAIN, PLAN_DUAL, PLAN_DH };
