@@ -12,10 +12,10 @@
 // and keeps the sums over rows (parameters, group gates) in registers: a block writes one partial row at its end, and one more launch adds the
 // partials in a fixed order.  No atomics: the same bits every run.
 //
-// Measured (kernel time): fp32 [29 952, 128], LayerNorm, scale: forward 11.8 us (61 MB, 5.2 TB/s), backward 19.1 + 5 us (92 MB); bf16 [16 384,
-// 4 096], post norm and a tanh gate per sample: forward 100 us (537 MB, 5.3 TB/s), backward 233 + 13 us (805 MB, 3.5 TB/s: two rows a CU in
-// flight at 222 registers a lane, four sums over 8 waves a row).  Loads a row ahead, no load under a branch (each is waited for before the next:
-// 264 -> 233 us), consecutive rows to a block so that a group's gate is read once (forward 161 -> 105 us).
+// Measured (kernel time): fp32 [29 952, 128], LayerNorm, scale: forward 12 us (61 MB, 5.1 TB/s), backward 19 + 5 us (92 MB, 4.8 TB/s); bf16
+// [16 384, 4 096], post norm and a tanh gate per sample: forward 98 us (537 MB, 5.5 TB/s), backward 215 + 8 us (805 MB, 3.7 TB/s: one row a CU
+// in flight, four sums over 8 waves a row).  Loads a row ahead, no load under a branch (each is waited for before the next: 264 -> 233 us),
+// consecutive rows to a block so that a group's gate is read once (forward 161 -> 105 us).
 #include "common.h"
 #include "elem.h"
 #include <initializer_list>
