@@ -14,9 +14,9 @@
 // Few tokens (up to 64): the weights are read once and nothing else matters; ffn_few_kernel streams them from memory into the matrix pipe's
 // operand layout without LDS, a block's 8 waves sharing the contraction.
 //
-// Measured (kernel time): bf16, T = 8 192, D = 2 048, F = 5 504: both projections 529 us (369 GFLOP, 698 TFLOP/s), the second matrix 238 us (776),
-// dg and du 474 us (390: 541 MB of g, u, dg and du go through its epilogue), dx 386 us (956), weight gradients 761 us (728).  fp32, T = 29 952,
-// D = 128, F = 512: 102, 40, 90, 68 and 60 us (44 to 198 TFLOP/s of fp32 work, three products each).  One token, bf16, D = 4 096,
+// Measured (kernel time): bf16, T = 8 192, D = 2 048, F = 5 504: both projections 549 us (369 GFLOP, 673 TFLOP/s), the second matrix 218 us (848),
+// dg and du 439 us (420: 541 MB of g, u, dg and du go through its epilogue), dx 369 us (1 001), weight gradients 722 us (767).  fp32, T = 29 952,
+// D = 128, F = 512: 102, 36, 91, 57 and 60 us (43 to 198 TFLOP/s of fp32 work, three products each).  One token, bf16, D = 4 096,
 // F = 11 008: 33 + 20 us (270 MB, 5.1 TB/s).
 #include "common.h"
 #include "elem.h"
@@ -288,12 +288,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm_kernel(GemmArgs args
     // where the registers hold them beside it (64 x 64), else behind it
     const bool inside = EPI == EPI_DH && m0 + BM <= a.M && n0 + BN <= a.N;
     uint4 gw[GJ][GM], uw[GJ][GM];
+    typedef unsigned w4 __attribute__((ext_vector_type(4), aligned(4)));
+    auto once = [&](const float *p) { return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const w4 *>(p))); };
     auto ask = [&](int j) {
 #pragma unroll
         for (int i = 0; i < GM; ++i) {
             const int64_t at = (int64_t)(m0 + (wm * TM + i) * 16 + (lane & 15)) * a.ldc + n0 + (wn * JN + j) * 16 + 4 * (lane >> 4);
-            gw[j][i] = Vec16<float>::raw(a.g + at);
-            uw[j][i] = Vec16<float>::raw(a.u + at);
+            gw[j][i] = once(a.g + at);
+            uw[j][i] = once(a.u + at);
         }
     };
     if (EARLY && inside)
@@ -380,6 +382,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm_kernel(GemmArgs args
         if (left >= 4) Vec16<float>::store(p, v);
         else for (int k = 0; k < left; ++k) p[k] = v[k];
     };
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    auto putn = [&](float *p, int left, const float *v) {
+        if (left >= 4) __builtin_nontemporal_store(f4u{v[0], v[1], v[2], v[3]}, reinterpret_cast<f4u *>(p));
+        else for (int k = 0; k < left; ++k) p[k] = v[k];
+    };
     auto getf = [&](const float *p, int left, float *v) {
         if (left >= 4) Vec16<float>::unpack(Vec16<float>::raw(p), v);
         else for (int k = 0; k < 4; ++k) v[k] = k < left ? p[k] : 0.f;
@@ -425,9 +432,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm_kernel(GemmArgs args
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] += b[k];
                 }
-                if (a.C2) {                                        // (kept in fp32: rounded to 16 bits they would double the gradients' error)
-                    putf(static_cast<float *>(a.C2) + at, left, v);
-                    putf(static_cast<float *>(a.C3) + at, left, w);
+                // (kept in fp32: rounded to 16 bits they would add a third to the gradients' error; past the caches, which then still hold h and,
+                // behind the product that reads g and u, dg and du for the next one: T = 29 952 in fp32 380 -> 348 us, T = 8 192, D = 2 048 in
+                // bf16 2 202 -> 2 151 us forward and backward; loads alone: 358, 2 172)
+                if (a.C2) {
+                    putn(static_cast<float *>(a.C2) + at, left, v);
+                    putn(static_cast<float *>(a.C3) + at, left, w);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
