@@ -3,6 +3,7 @@ around a block with its gate and residual scale (csrc/residual_norm.hip).  They 
 (nmrf/models/NMP.py:337, 537, 675), its block tails, x + proj(attn) / x + mlp(norm2(x)) (NMP.py:337-364), their post-norm form
 (NMP.py:366-382) and stochastic depth (nmrf/models/swin.py:228-233, 300-301)."""
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import kernels as K
@@ -36,17 +37,21 @@ def refuse_captured_backward(name):
 
 
 def differentiated(*tensors):
-    """Whether a backward pass may follow (a Function does not see that gradients are switched off)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its Function.  A backward pass may follow (a Function does not see that gradients are switched off); or a
+    forward-mode derivative is being taken, which the kernels alone would drop and the Function refuses; or a trace is being recorded, which
+    holds a Function as one node and of the kernels alone nothing but the allocation of their outputs."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or forward_ad._current_level >= 0 or torch.jit.is_tracing()
 
 
 class ResidualNormFn(torch.autograd.Function):
+    # (checks and layout belong to the forward pass: a recorded trace calls it again, with tensors of other sizes)
     @staticmethod
-    def forward(ctx, x, y, gate, scale, post_w, post_b, next_w, next_b, spec):
-        ctx.save_for_backward(x, y, gate, scale, post_w, post_b, next_w, next_b)
+    def forward(ctx, *call):
+        args, spec = _norm_call(*call)
+        ctx.save_for_backward(*args)
         ctx.spec = spec
         ctx.set_materialize_grads(False)
-        out, h = K.residual_norm(x, y, gate, scale, post_w, post_b, next_w, next_b, spec)
+        out, h = K.residual_norm(*args, spec)
         return (out, h) if spec.next else out
 
     @staticmethod
@@ -61,18 +66,51 @@ class ResidualNormFn(torch.autograd.Function):
         return (*K.residual_norm_backward(*saved, d_out, d_h, ctx.spec, want), None)
 
 
+def _sizes(t):
+    return tuple(t.shape)                                           # (while a trace is being recorded its entries are tensors: int() where one is kept)
+
+
 def _gate_layout(x, gate):
-    """(rows that share a gate row, 1 or C) of a gate that broadcasts over x from some dimension on; the gate as rows."""
-    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
-    lead, c = x.shape[:-1], x.shape[-1]
-    keep = next((k for k in range(len(lead) + 1) if shape[:k] == tuple(lead[:k]) and all(n == 1 for n in shape[k:-1])), None)
-    if gate.dim() > x.dim() or gate.dim() < 1 or shape[-1] not in (1, c) or keep is None:
+    """(rows that share a gate row, 1 or C) of a gate of shape `gate` that broadcasts over shape `x` from some dimension on."""
+    shape = (1,) * (len(x) - len(gate)) + gate
+    lead, c = x[:-1], x[-1]
+    keep = next((k for k in range(len(lead) + 1) if shape[:k] == lead[:k] and all(n == 1 for n in shape[k:-1])), None)
+    if len(gate) > len(x) or len(gate) < 1 or shape[-1] not in (1, c) or keep is None:
         raise ValueError("residual_norm: a gate of shape %s does not share one row with whole trailing dimensions of %s: its leading dimensions "
-                         "are x's up to some point and 1 behind it, its last one %d or 1" % (tuple(gate.shape), tuple(x.shape), c))
+                         "are x's up to some point and 1 behind it, its last one %d or 1" % (gate, x, c))
     rows = 1
     for n in lead[keep:]:
-        rows *= n
-    return max(rows, 1), shape[-1]
+        rows *= int(n)
+    return max(rows, 1), int(shape[-1])
+
+
+def _norm_call(x, y, gate, vec, post_w, post_b, next_w, next_b, options):
+    """residual_norm's arguments checked: the contiguous tensors, and the call's numbers."""
+    kind, gate_act, scale_value, post, nxt, eps = options
+    shape = _sizes(x)
+    if shape != _sizes(y) or not shape:
+        raise ValueError("residual_norm: x %s and y %s differ" % (shape, _sizes(y)))
+    c = int(shape[-1])
+    if not 1 <= c <= 8192:
+        raise ValueError("residual_norm: %d channels are not in 1 ... 8192" % c)
+    check_rows("residual_norm", ("x", "y", "gate"), (x, y, gate))
+    device, of = x.device, None                                         # of: the parameters' type
+    params = (vec, post_w, post_b, next_w, next_b)
+    for k, t in zip(("scale", "post_weight", "post_bias", "next_weight", "next_bias"), params):
+        if t is None:
+            continue
+        if _sizes(t) != (c,):
+            raise ValueError("residual_norm: %s has shape %s, expected (%d,)" % (k, _sizes(t), c))
+        if t.device != device or not t.is_contiguous():
+            raise NmrfHipError("residual_norm: %s is not a contiguous tensor on %s" % (k, device))
+        if of is None:
+            of = t.dtype
+        if t.dtype != of or (of != x.dtype and of != torch.float32):
+            raise NmrfHipError("residual_norm: weights, biases and the scale vector are all %s or all torch.float32, got %s for %s" % (x.dtype, t.dtype, k))
+    rows, cols = _gate_layout(shape, _sizes(gate)) if gate is not None else (1, 1)
+    spec = K.ResidualNormSpec(int(x.numel()) // c, c, int(kind == "rms"), eps, rows, cols, _GATE_ACTS[gate_act], scale_value, int(post), int(nxt),
+                              int(of == torch.float32), K.DTYPE_CODE[x.dtype])
+    return (x.contiguous(), y.contiguous(), None if gate is None else gate.contiguous(), *params), spec
 
 
 def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None, scale=None, kind="layer", eps=1e-5):
@@ -89,40 +127,18 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
         raise ValueError("residual_norm: kind is 'layer' or 'rms', got %r" % (kind,))
     if gate_act not in _GATE_ACTS:
         raise ValueError("residual_norm: gate_act is None, 'sigmoid' or 'tanh', got %r" % (gate_act,))
-    shape = x.shape
-    if shape != y.shape or not shape:
-        raise ValueError("residual_norm: x %s and y %s differ" % (tuple(shape), tuple(y.shape)))
     if not eps >= 0:
         raise ValueError("residual_norm: eps %r" % (eps,))
-    c = shape[-1]
-    if not 1 <= c <= 8192:
-        raise ValueError("residual_norm: %d channels are not in 1 ... 8192" % c)
     post_w, post_b = post_norm if post_norm is not None else (None, None)
     next_w, next_b = next_norm if next_norm is not None else (None, None)
     vec = scale if isinstance(scale, torch.Tensor) else None
-    check_rows("residual_norm", ("x", "y", "gate"), (x, y, gate))
-    device, of = x.device, None                                         # of: the parameters' type
-    params = (vec, post_w, post_b, next_w, next_b)
-    for k, t in zip(("scale", "post_weight", "post_bias", "next_weight", "next_bias"), params):
-        if t is None:
-            continue
-        if t.shape != (c,):
-            raise ValueError("residual_norm: %s has shape %s, expected (%d,)" % (k, tuple(t.shape), c))
-        if t.device != device or not t.is_contiguous():
-            raise NmrfHipError("residual_norm: %s is not a contiguous tensor on %s" % (k, device))
-        if of is None:
-            of = t.dtype
-        if t.dtype != of or (of != x.dtype and of != torch.float32):
-            raise NmrfHipError("residual_norm: weights, biases and the scale vector are all %s or all torch.float32, got %s for %s" % (x.dtype, t.dtype, k))
-    rows, cols = _gate_layout(x, gate) if gate is not None else (1, 1)
-    s = K.ResidualNormSpec(x.numel() // c, c, int(kind == "rms"), float(eps), rows, cols, _GATE_ACTS[gate_act],
-                           1.0 if scale is None or vec is not None else float(scale), int(post_norm is not None), int(next_norm is not None),
-                           int(of == torch.float32), K.DTYPE_CODE[x.dtype])
-    args = (x.contiguous(), y.contiguous(), None if gate is None else gate.contiguous(), *params)
-    if differentiated(*args):
-        return ResidualNormFn.apply(*args, s)
-    out, h = K.residual_norm(*args, s)
-    return (out, h) if s.next else out
+    tensors = (x, y, gate, vec, post_w, post_b, next_w, next_b)
+    options = (kind, gate_act, 1.0 if scale is None or vec is not None else float(scale), post_norm is not None, next_norm is not None, float(eps))
+    if differentiated(*tensors):
+        return ResidualNormFn.apply(*tensors, options)
+    args, spec = _norm_call(*tensors, options)
+    out, h = K.residual_norm(*args, spec)
+    return (out, h) if spec.next else out
 
 
 _FFN_ACTS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -131,17 +147,36 @@ _FFN_NAMES = ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
 
 class GatedFfnFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        y, h, g, u, amax = K.gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, h, g, u, amax)
-        ctx.act = act
+    def forward(ctx, *call):
+        args = _ffn_call(*call[:7])
+        ctx.act, ctx.shape = _FFN_ACTS[call[7]], _sizes(call[0])
+        y, h, g, u, amax = K.gated_ffn(*args, ctx.act, any(ctx.needs_input_grad))
+        ctx.save_for_backward(*args[:4], h, g, u, amax)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         refuse_captured_backward("gated_ffn")
-        return (*K.gated_ffn_backward(*ctx.saved_tensors, dy.contiguous(), ctx.act, ctx.needs_input_grad[:7]), None)
+        dx, *rest = K.gated_ffn_backward(*ctx.saved_tensors, dy.contiguous(), ctx.act, ctx.needs_input_grad[:7])
+        return (None if dx is None else dx.view(ctx.shape), *rest, None)
+
+
+def _ffn_call(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
+    """gated_ffn's tensors checked: contiguous, x as rows."""
+    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2:
+        raise ValueError("gated_ffn: x [..., D], w_gate, w_up [F, D], w_down [D', F]; got %s, %s, %s" % (_sizes(x), _sizes(w_gate), _sizes(w_down)))
+    d, f, do = int(x.shape[-1]), int(w_gate.shape[0]), int(w_down.shape[0])
+    for name, t, want in zip(_FFN_NAMES[1:], (w_gate, w_up, w_down, b_gate, b_up, b_down), ((f, d), (f, d), (do, f), (f,), (f,), (do,))):
+        if t is not None and _sizes(t) != want:
+            raise ValueError("gated_ffn: %s has shape %s, expected %s" % (name, _sizes(t), want))
+    if min(d, f, do) < 1 or max(d, f, do) > 1 << 22:
+        raise ValueError("gated_ffn: widths %d, %d, %d are not in 1 ... 2^22" % (d, f, do))
+    check_rows("gated_ffn", _FFN_NAMES, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
+    rows = int(x.numel()) // d
+    if rows > 0x7fffffff - 256:
+        raise ValueError("gated_ffn: %d rows" % rows)
+    return [None if t is None else t.contiguous() for t in (x.reshape(rows, d), w_gate, w_up, w_down, b_gate, b_up, b_down)]
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act="silu"):
@@ -155,19 +190,6 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act=
     (decoding) stream the weights once.  The forward pass may be captured into a graph, the backward pass may not (it raises)."""
     if act not in _FFN_ACTS:
         raise ValueError("gated_ffn: act is 'silu', 'gelu' or 'relu', got %r" % (act,))
-    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2:
-        raise ValueError("gated_ffn: x [..., D], w_gate, w_up [F, D], w_down [D', F]; got %s, %s, %s" % (
-            tuple(x.shape), tuple(w_gate.shape), tuple(w_down.shape)))
-    d, (f, do) = x.shape[-1], (w_gate.shape[0], w_down.shape[0])
-    for name, t, shape in zip(_FFN_NAMES[1:], (w_gate, w_up, w_down, b_gate, b_up, b_down), ((f, d), (f, d), (do, f), (f,), (f,), (do,))):
-        if t is not None and t.shape != shape:
-            raise ValueError("gated_ffn: %s has shape %s, expected %s" % (name, tuple(t.shape), shape))
-    if min(d, f, do) < 1 or max(d, f, do) > 1 << 22:
-        raise ValueError("gated_ffn: widths %d, %d, %d are not in 1 ... 2^22" % (d, f, do))
-    check_rows("gated_ffn", _FFN_NAMES, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
-    rows = x.numel() // d
-    if rows > 0x7fffffff - 256:
-        raise ValueError("gated_ffn: %d rows" % rows)
-    args = [None if t is None else t.contiguous() for t in (x.reshape(rows, d), w_gate, w_up, w_down, b_gate, b_up, b_down)]
-    y = GatedFfnFn.apply(*args, _FFN_ACTS[act]) if differentiated(*args) else K.gated_ffn(*args, _FFN_ACTS[act], False)[0]
-    return y.view(*x.shape[:-1], do)
+    tensors = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    y = GatedFfnFn.apply(*tensors, act) if differentiated(*tensors) else K.gated_ffn(*_ffn_call(*tensors), _FFN_ACTS[act], False)[0]
+    return y.view(*x.shape[:-1], y.shape[-1])
