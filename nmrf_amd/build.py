@@ -41,9 +41,9 @@ def _sources(debug=False):
 
 def source_stamp():
     """sha256/16 over every source and header a library is built from (names + contents, both libraries hash the same set: the
-    tools library is a superset build of the same tree)."""
+    tools library is a superset build of the same tree) and the compiler flags that both share."""
     import hashlib
-    h = hashlib.sha256()
+    h = hashlib.sha256("\0".join(FLAGS).encode())
     files = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h")) and not f.startswith("_ab_"))
     files += [os.path.join(os.path.dirname(HERE), "include", f) for f in ("nmrf_hip.h", "nmrf_hip_debug.h")]
     for f in files:
@@ -89,6 +89,12 @@ def build_library(force=False, verbose=True, debug=False):
     stamp = source_stamp()
     stamp_file = os.path.join(objdir, "build_stamp.txt")
     old_stamp = open(stamp_file).read().strip() if os.path.exists(stamp_file) else None
+    # the flags the objects here were compiled with; absent while a build with other flags is under way, so that one cut short begins again
+    flags_file = os.path.join(objdir, "build_flags.txt")
+    if not os.path.exists(flags_file) or open(flags_file).read() != "\n".join(flags):
+        force = True
+        if os.path.exists(flags_file):
+            os.remove(flags_file)
     for src in _sources(debug):
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
@@ -113,6 +119,8 @@ def build_library(force=False, verbose=True, debug=False):
                     raise RuntimeError("hipcc failed: %s\n%s" % (" ".join(cmd), log))
     with open(stamp_file, "w") as f:
         f.write(stamp + "\n")
+    with open(flags_file, "w") as f:
+        f.write("\n".join(flags))
     stale_lib = not os.path.exists(lib_path) or any(os.path.getmtime(o) > os.path.getmtime(lib_path) for o in objs)
     if jobs or stale_lib:
         cmd = [hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", lib_path] + objs
