@@ -42,8 +42,10 @@ class AdamW(torch.optim.Optimizer):
         return s
 
     def moments(self, p):
-        """(first, second) moment of parameter p as fp32 tensors, whatever they are held in."""
-        s = self.state[p]
+        """(first, second) moment of parameter p as fp32 tensors, whatever they are held in.  A parameter that has taken no step has none (KeyError)."""
+        s = self.state.get(p)                                          # (a lookup by [p] would leave an empty entry behind)
+        if not s:
+            raise KeyError("AdamW: a parameter of shape %s has taken no step" % (tuple(p.shape),))
         if "exp_avg_scale" in s:
             return adamw_moment(s["exp_avg"], s["exp_avg_scale"]), adamw_moment(s["exp_avg_sq"], s["exp_avg_sq_scale"], squared=True)
         return s["exp_avg"], s["exp_avg_sq"]
@@ -115,7 +117,7 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self):
         sd = super().state_dict()
-        sd["state"] = {k: {**s, "step": torch.tensor(float(s["step"]))} for k, s in sd["state"].items()}
+        sd["state"] = {k: {**s, "step": torch.tensor(float(s["step"]))} for k, s in sd["state"].items() if s}
         return sd
 
     def load_state_dict(self, state_dict):
