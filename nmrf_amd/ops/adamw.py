@@ -32,9 +32,9 @@ def _addr(a):
 class AdamWPlan:
     """What a training program keeps for one list of parameters that step together: the checked tensors and the host tables the launch reads.
 
-    params: CUDA tensors of one device and one type (fp32, bf16, fp16), contiguous, no tensor twice.  exp_avgs, exp_avg_sqs: fp32 tensors of
+    params: CUDA tensors of one device and one type (fp32, bf16, fp16), contiguous, none that overlap.  exp_avgs, exp_avg_sqs: fp32 tensors of
     the same sizes, or uint8 ones with exp_avg_scales, exp_avg_sq_scales (fp32, one per started 256 elements): moments in 8 bits, zeros to
-    begin with.  weight_decay: one number, or one for each parameter.
+    begin with; no storage is shared.  weight_decay: one number, or one for each parameter.
 
         norm = plan.step(grads, step=t, lr=..., max_norm=1.0)
 
@@ -71,6 +71,13 @@ class AdamWPlan:
         self._tables = [np.fromiter(map(_data_ptr, x), np.uint64, n) for x in self._lists]
         if len(set(self._tables[0][self._numel > 0].tolist())) != int(np.sum(self._numel > 0)):
             raise NmrfHipError("AdamWPlan: a parameter is in the list twice")
+        # (each tensor is updated in place by blocks of its own: none may reach into another)
+        start = np.concatenate(self._tables)
+        size = np.concatenate([np.fromiter(map(_numel, x), np.uint64, n) * np.uint64(x[0].element_size()) for x in self._lists])
+        order = np.argsort(start[size > 0], kind="stable")
+        start, end = start[size > 0][order], (start + size)[size > 0][order]
+        if bool((end[:-1] > start[1:]).any()):
+            raise NmrfHipError("AdamWPlan: parameters or moments share storage")
         # (a parameter's address is checked each step; the moments' storage is held, whatever becomes of the tensors)
         self._held = [list(map(torch.Tensor.detach, x)) for x in self._lists[1:]]
         self._g = np.zeros(n, np.uint64)
