@@ -62,3 +62,18 @@ def test_a_build_cut_short_begins_again(tree, monkeypatch):
     monkeypatch.setattr(build, "FLAGS", ["-O3", "-first"])          # back to the first flags: a.o may be of the second ones
     assert run() == {"a.o", "b.o", "build_stamp.o"}
     assert all("-first" in f.read_text() for f in (root / "obj").glob("*.o"))
+
+
+def test_tools_compile_with_the_products_flags():
+    """What the tools compare with the product is compiled with its flags: every hipcc line that takes a source."""
+    tools = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools")
+    seen = 0
+    for name in sorted(os.listdir(tools)):
+        if not name.endswith((".sh", ".py")):
+            continue
+        with open(os.path.join(tools, name)) as f:
+            for line in f:
+                if "bin/hipcc" in line and (".hip" in line.replace("libnmrf_hip", "") or "src]" in line):
+                    seen += 1
+                    assert "$FLAGS" in line or "*FLAGS" in line, (name, line)
+    assert seen >= 6

@@ -6,7 +6,7 @@ cd "$(dirname "$0")/.." || exit 1
 set -e
 name=$1; extra=$2; shift 2
 mkdir -p nmrf_amd/lib/ab_$name nmrf_amd/build_ab/$name
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function"
+FLAGS="$(python3 -c 'from nmrf_amd.build import FLAGS; print(*FLAGS)')"        # the product's own, whatever is compared
 for f in "$@"; do
   /opt/rocm/bin/hipcc $FLAGS $extra -c nmrf_amd/csrc/$f.hip -o nmrf_amd/build_ab/$name/$f.o &
 done

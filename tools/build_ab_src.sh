@@ -6,6 +6,7 @@ set -e
 name=$1; rev=$2; shift 2
 python -m nmrf_amd.build --main-only > /dev/null
 mkdir -p nmrf_amd/lib/ab_$name nmrf_amd/build_ab/$name
+FLAGS="$(python3 -c 'from nmrf_amd.build import FLAGS; print(*FLAGS)')"        # the product's own, whatever is compared
 objs=""
 for o in nmrf_amd/build/*.o; do
   b=$(basename $o .o); skip=0
@@ -15,7 +16,7 @@ done
 for f in "$@"; do
   b=$(basename $f .hip)
   git show $rev:nmrf_amd/csrc/$f > nmrf_amd/csrc/_ab_$b.hip
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -c nmrf_amd/csrc/_ab_$b.hip -o nmrf_amd/build_ab/$name/$b.o
+  /opt/rocm/bin/hipcc $FLAGS -c nmrf_amd/csrc/_ab_$b.hip -o nmrf_amd/build_ab/$name/$b.o
   rm nmrf_amd/csrc/_ab_$b.hip
   objs="$objs nmrf_amd/build_ab/$name/$b.o"
 done

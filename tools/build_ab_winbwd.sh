@@ -3,7 +3,7 @@
 # nmrf_amd/lib/ab_wb<k>/libnmrf_hip.so, for tools/winbwd_phase_bench.py.  Run after `python -m nmrf_amd.build`.
 cd "$(dirname "$0")/.." || exit 1
 set -e
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function"
+FLAGS="$(python3 -c 'from nmrf_amd.build import FLAGS; print(*FLAGS)')"        # the product's own, whatever is compared
 for k in 0 1 2 3 4; do
   mkdir -p nmrf_amd/lib/ab_wb$k nmrf_amd/build_wb
   ( /opt/rocm/bin/hipcc $FLAGS -DWB_STOP=$k -c nmrf_amd/csrc/backward.hip -o nmrf_amd/build_wb/backward_$k.o

@@ -22,6 +22,7 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 from nmrf_amd import kernels as K  # noqa: E402
+from nmrf_amd.build import FLAGS  # noqa: E402
 from nmrf_amd.utils.hashinit import unit_noise  # noqa: E402
 
 ap = argparse.ArgumentParser()
@@ -45,7 +46,7 @@ def build_so():
     src, so = os.path.join(ROOT, "tools/ab/mlp_b32.hip"), os.path.join(ROOT, args.so)
     if not os.path.exists(so):
         os.makedirs(os.path.dirname(so), exist_ok=True)
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-o", so, src])
+        subprocess.check_call(["/opt/rocm/bin/hipcc", *FLAGS, "-shared", "-o", so, src])
     lib = ctypes.CDLL(so)
     lib.mlp_b32_f32.restype = ctypes.c_int
     return lib
