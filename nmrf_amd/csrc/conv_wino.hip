@@ -144,7 +144,7 @@ __global__ __launch_bounds__(512, 4) void conv3x3_wino_kernel(const float *__res
 #pragma unroll 1
         for (int m = 0; m < 2; ++m) {                               // (unrolled, both patches are fetched up front: spills)
             const float *rp = buf + r_off + (2 * q + m) * 6 * WN_RS;
-            // patch rows as two packed halves (columns 01 | 23); V = B^T d B with v_pk_add_f32
+            // patch rows as two packed halves (columns 01 | 23); V = B^T d B on two-wide values
             f32x2 dl[4], dh[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {

@@ -111,17 +111,17 @@ extern "C" int nmrf_cost_volume_f32(const float *f1, const float *f2, int B, int
 
 // ------------------------------------------------------------------------------------------------
 // A3: Conv1d(G->8)-ReLU-Conv1d(8->16)-ReLU-Conv1d(16->1) along D (k=5, zero pad 2) + softmax.
-// One wave = TWO pixels, lane = disparity bin: the two pixels are the two halves of a packed fp32 FMA
-// (two IEEE fmas, one per pixel, same (channel, tap) order as the scalar form -> same bits), the
-// weight is a wave-uniform SGPR broadcast to both halves, so the weights are read in their reference
+// One wave = TWO pixels, lane = disparity bin: the two pixels are the two halves of a two-wide fp32 value
+// (two v_fma_f32 a step, one per pixel, same (channel, tap) order as the one-pixel form -> same bits), the
+// weight is a wave-uniform SGPR given to both, so the weights are read in their reference
 // layout and in memory order (s_load_dwordx16), once per two pixels.  Activations go through a
 // wave-private LDS strip [ch][2+64+2] of pixel pairs (zero guard cells realise the padding; one 8-byte
 // read per tap); softmax max/sum are wave shuffles.  Nothing is shared between waves: every ordering
 // point is a wave-level one.
 // (One pixel per wave with scalar v_fmac and SGPR weights: 5 400 cycles per pixel -- a wave64 v_fma_f32 with an SGPR operand
-// issues every 5.3 cycles on this chip, against 2.9 with VGPR operands and 4.9 for v_pk_fma_f32 with either; measured,
-// profiles/r03s_filter_ab.txt.  This form: 7 400 cycles per PAIR of pixels, unroll / block shape / reduction style make no
-// difference.)
+// issues every 5.3 cycles on this chip, against 2.9 with VGPR operands; measured, profiles/r03s_filter_ab.txt.  This form with
+// packed FMAs, which the library is no longer compiled with: 7 400 cycles per PAIR of pixels, unroll / block shape / reduction
+// style make no difference.)
 // ------------------------------------------------------------------------------------------------
 #define FS_WPB 4   // waves per block
 #define FS_LD 68

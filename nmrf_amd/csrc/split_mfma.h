@@ -84,8 +84,8 @@ __device__ __forceinline__ void split2u(f32x2 a, h16x2 &hi, h16x2 &lo) {
         lo = __builtin_bit_cast(h16x2, l);
     }
 #elif defined(NMRF_SCALAR_SPLIT)
-    // A/B build (tools/build_ab_nopk.sh): the same two subtractions as plain v_sub_f32 instead of one v_pk_add_f32 -- a packed fp32
-    // instruction beside MFMAs costs more than its issue slot (MI355X_MICROARCH.md, "price of one filler beside MFMAs")
+    // A/B build (tools/build_ab_nopk.sh): the same two subtractions written one by one.  (Compiled to one v_pk_add_f32 they cost more than its
+    // issue slot beside MFMAs; the library is built without packed fp32 now, nmrf_amd/build.py)
     const float b0 = (float)hi[0], b1 = (float)hi[1];
     const float l0 = a[0] - b0, l1 = a[1] - b1;
     lo = h16x2{(_Float16)l0, (_Float16)l1};

@@ -351,8 +351,8 @@ struct WinFastLds {
 // lanes of a block are the four labels of ONE pixel -- they need the same 36 table rows -- so block b multiplies (4 key pixels x 4
 // channels of the table rows rel(P_b, .)) by (4 channels x the pixel's 4 tokens): lane j ends up with its own token's dot products
 // for 4 key pixels, accumulated over the 8 channel chunks.  Split fp16 operands (3 products, table scaled by 2^10 so that its low
-// parts are normal fp16 numbers).  Per lane and phase: 144 ds_read_b64 + 216 of these 8-cycle MFMAs instead of 288 ds_read_b128 + 576
-// v_pk_fma_f32 -- the VALU form was bound by the LDS (11.5k array cycles per block of ten waves for the table rows, of a 12.4k phase).
+// parts are normal fp16 numbers).  Per lane and phase: 144 ds_read_b64 + 216 of these 8-cycle MFMAs instead of 288 ds_read_b128 + 1152
+// v_fma_f32 -- the VALU form was bound by the LDS (11.5k array cycles per block of ten waves for the table rows, of a 12.4k phase).
 template <int NKT, int WIN, int NL, int WPB, int OCC, bool TIMED = false, int PK = 1, bool KV16 = false, bool P0M = false, bool QAL = false>
 __global__ __launch_bounds__(64 * NKT * WPB, OCC) void window_attn_fast_kernel(const float *__restrict__ qkv,
         const float *__restrict__ table, WinGeom g, float scale, float *__restrict__ out,
