@@ -39,9 +39,9 @@ __device__ __forceinline__ f32x4 mma(const uint4 &a, const uint4 &b, f32x4 c, __
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// act(g) and its derivative.  gelu: Phi(g) from erfc(|g| / sqrt 2) = 2^(-t P(t)), t = |g| <= 7, the polynomial of gelu_fast (common.h: off by
-// 5.3e-8 in Phi's scale), one more exponential for the density in the derivative.  Beyond 7 both are zero (Phi < 1.3e-12): held there, they
-// would come back times any |g|.
+// act(g) and its derivative.  gelu: Phi(g) from erfc(|g| / sqrt 2) = 2^(-t P(t)), t = min(|g|, 7), the polynomial of gelu_fast (common.h: off by
+// 5.3e-8 in Phi's scale), one more exponential for the density in the derivative.  Below -7 the value is zero (g Phi(g) > -9e-12; Phi held at
+// its value at -7 would come back times any g), the slope held (-6e-11).
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ void act_both(float g, int act, float &value, float &slope) {
@@ -50,16 +50,15 @@ __device__ __forceinline__ void act_both(float g, int act, float &value, float &
         value = g == -INFINITY ? 0.f : g * s;
         slope = fmaf(value, 1.0f - s, s);
     } else if (act == ACT_GELU) {
-        const bool far = fabsf(g) > 7.0f;
         const float t = fminf(fabsf(g), 7.0f);
         float p = fmaf(-3.0177725420799106e-05f, t, 0.0007414184510707855f);
         p = fmaf(p, t, -0.007980725727975368f);
         p = fmaf(p, t, 0.053240980952978134f);
         p = fmaf(p, t, 0.45891475677490234f);
         p = fmaf(p, t, 1.151147484779358f);
-        const float half = far ? 0.f : 0.5f * __builtin_amdgcn_exp2f(-t * p), phi = g < 0.f ? half : 1.0f - half;
-        value = g == -INFINITY ? 0.f : g * phi;
-        slope = far ? phi : fmaf(t * (g < 0.f ? -0.39894228040143267794f : 0.39894228040143267794f), exp_of(-0.5f * t * t), phi);
+        const float half = 0.5f * __builtin_amdgcn_exp2f(-t * p), phi = g < 0.f ? half : 1.0f - half;
+        value = g < -7.0f ? 0.f : g * phi;
+        slope = fmaf(t * (g < 0.f ? -0.39894228040143267794f : 0.39894228040143267794f), exp_of(-0.5f * t * t), phi);
         if (g != g) value = slope = g;
     } else {
         value = g > 0.f ? g : (g != g ? g : 0.f);
