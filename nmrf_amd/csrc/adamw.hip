@@ -10,8 +10,9 @@
 // table in device memory, no copy and no lifetime rule; a block owns 4 096 elements of one tensor and finds it by one ballot over the list.
 //
 // Bound by memory: p, m and v in and out, g in (and once more for the norm).  Measured, 202 M elements: bf16 with 32-bit moments 806 us (4.45 GB,
-// 5.5 TB/s), the norm before it 126 us (0.40 GB, 3.2 TB/s); fp32 with 8-bit moments 832 us (3.25 GB, 3.9 TB/s), reading a moment out 204 us
-// (1.01 GB, 4.9 TB/s).  A model of 180 tensors and 3 M elements: 3 x 5.7 us with 32-bit moments, 4 x 9.6 us with 8-bit ones, 9 us for the norm.
+// 5.5 TB/s), the norm before it 126 us (0.40 GB, 3.2 TB/s); fp32 with 8-bit moments 822 us (3.25 GB, 4.0 TB/s), bf16 with 8-bit moments 753 us
+// (2.03 GB, 2.7 TB/s: the rounding's VALU work is that of fp32), reading a moment out 204 us (1.01 GB, 4.9 TB/s).  A model of 180 tensors and
+// 3 M elements: 3 x 5.7 us with 32-bit moments, 4 x 9.8 us with 8-bit ones, 9 us for the norm.
 #include "common.h"
 #include "elem.h"
 #include <algorithm>

@@ -17,7 +17,8 @@
 // Measured (kernel time): bf16, T = 8 192, D = 2 048, F = 5 504: both projections 549 us (369 GFLOP, 673 TFLOP/s), the second matrix 218 us (848),
 // dg and du 439 us (420: 541 MB of g, u, dg and du go through its epilogue), dx 369 us (1 001), weight gradients 722 us (767).  fp32, T = 29 952,
 // D = 128, F = 512: 102, 36, 91, 57 and 60 us (43 to 198 TFLOP/s of fp32 work, three products each).  One token, bf16, D = 4 096,
-// F = 11 008: 33 + 20 us (270 MB, 5.1 TB/s).
+// F = 11 008: 33 + 20 us (270 MB, 5.1 TB/s); 16 tokens 39 + 29, 64 tokens 81 + 62; in fp32 one token 70 + 41 (541 MB, 4.9 TB/s), 64 tokens
+// 203 + 132 (four k steps of v_mfma_f32_16x16x4_f32 for every 16-byte load).
 #include "common.h"
 #include "elem.h"
 #include <algorithm>
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ffn_gemm_kernel(GemmArgs args
                     for (int k = 0; k < 4; ++k) w[k] += b[k];
                 }
                 // (kept in fp32: rounded to 16 bits they would add a third to the gradients' error; past the caches, which then still hold h and,
-                // behind the product that reads g and u, dg and du for the next one: T = 29 952 in fp32 380 -> 348 us, T = 8 192, D = 2 048 in
+                // behind the product that reads g and u, dg and du for the next one: T = 29 952 in fp32 380 -> 348 us (350 ... 361 since, by the caches), T = 8 192, D = 2 048 in
                 // bf16 2 202 -> 2 151 us forward and backward; loads alone: 358, 2 172)
                 if (a.C2) {
                     putn(static_cast<float *>(a.C2) + at, left, v);

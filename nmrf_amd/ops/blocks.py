@@ -30,8 +30,9 @@ def check_rows(name, names, tensors):
 
 
 def refuse_captured_backward(name):
-    """A captured backward pass accumulates into leaves on the stream their first graph was built on; with an eager graph of the same leaves
-    alive that is another stream, and the capture takes the process down.  Forward passes are captured freely."""
+    """A captured backward pass that accumulates into leaves does so on the stream their first graph was built on; with an eager graph of the same
+    leaves alive that is another stream, and the capture takes the process down.  Whether a pass goes on to leaves or returns its gradients
+    (torch.autograd.grad) cannot be seen from a node of it: all are refused.  Forward passes are captured freely."""
     if torch.cuda.is_current_stream_capturing():
         raise NmrfHipError("%s: a backward pass is not captured into a graph (capture the forward pass, or run it eagerly)" % name)
 
@@ -121,8 +122,8 @@ def residual_norm(x, y, next_norm=None, post_norm=None, gate=None, gate_act=None
     may be None; kind "layer" or "rms".  gate: broadcasts over x with x's leading dimensions up to some point and 1 behind it -- [..., C] per
     element, [..., 1] per row, [B, 1, C] or [B, 1, 1] per sample (conditioned blocks, stochastic depth: zeros and 1 / keep) --, through
     gate_act None, "sigmoid" or "tanh".  scale: a number, or a vector over the channels.  Weights, biases and the scale vector are all in x's
-    type or all in fp32.  Differentiable in every tensor; statistics and sums in fp32, the same bits every run.  The forward pass may be
-    captured into a graph, the backward pass may not (it raises)."""
+    type or all in fp32.  Differentiable in every tensor, once and backwards (forward mode raises); statistics and sums in fp32, the same bits
+    every run.  The forward pass may be captured into a graph or recorded by torch.jit.trace, the backward pass may not be captured (it raises)."""
     if kind not in ("layer", "rms"):
         raise ValueError("residual_norm: kind is 'layer' or 'rms', got %r" % (kind,))
     if gate_act not in _GATE_ACTS:
@@ -186,10 +187,12 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act=
     second matrix in another.
 
     x: [..., D]; w_gate, w_up: [F, D]; w_down: [D', F]; biases [F], [F], [D'], each may be None; one type, fp32 / bf16 / fp16 (copied where not
-    contiguous).  act: "silu", "gelu" (erf) or "relu".  16-bit types multiply on the matrix pipe as they are (sums in fp32; h is kept in the
-    type, both projections for the backward pass in fp32); fp32 is multiplied as scaled fp16 pairs: errors of 2^-22 relative to each operand's
-    largest entry, and an infinite input gives NaN.  Differentiable in every tensor, the same bits every run.  Up to 64 rows without gradients
-    (decoding) stream the weights once.  The forward pass may be captured into a graph, the backward pass may not (it raises)."""
+    contiguous; autocast does not cast here).  act: "silu", "gelu" (erf; zero below -7) or "relu".  16-bit types multiply on the matrix pipe as
+    they are, sums in fp32; h and the gradients of both projections are rounded to the type on the way, as operands of the next product, the
+    projections are kept in fp32 for the backward pass.  fp32 is multiplied as scaled fp16 pairs: errors of 2^-22 of a value and 2^-38 of the largest
+    entry that shares its scale (w_gate with w_up, the gradients of both projections), and an infinite input gives NaN.  Differentiable in every
+    tensor, once and backwards (forward mode raises), the same bits every run.  Up to 64 rows without gradients (decoding) stream the weights
+    once.  The forward pass may be captured into a graph or recorded by torch.jit.trace, the backward pass may not be captured (it raises)."""
     if act not in _FFN_ACTS:
         raise ValueError("gated_ffn: act is 'silu', 'gelu' or 'relu', got %r" % (act,))
     tensors = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)

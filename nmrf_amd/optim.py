@@ -10,7 +10,7 @@ from .ops.adamw import AdamWPlan, adamw_moment, clip_factor, refuse_capture
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW(params, lr, betas, eps, weight_decay) with decoupled weight decay, on CUDA parameters in fp32, bf16 or fp16.
+    """AdamW(params, lr, betas, eps, weight_decay) with decoupled weight decay, on contiguous CUDA parameters in fp32, bf16 or fp16 (others raise).
 
     state_bits=32: state and checkpoints as torch.optim.AdamW's ({'step', 'exp_avg', 'exp_avg_sq'}): either loads the other's.
     state_bits=8: tensors of min_8bit_size elements or more hold their moments as uint8 codes with a fp32 scale for 256 elements (2.03 bytes a
@@ -19,7 +19,8 @@ class AdamW(torch.optim.Optimizer):
 
     step(max_norm=c) clips the global gradient norm on the way (torch.nn.utils.clip_grad_norm_'s factor, applied as the gradients are read:
     .grad itself is not rewritten) and leaves the norm in self.grad_norm, a 0-dim device tensor.  Parameters whose .grad is None are skipped,
-    as in torch.  A step is not captured into a graph (it raises): lr and the step count are numbers of the host."""
+    as in torch; a step whose set of parameters with gradients is another one than the last step's checks and lists them anew.  A step is not
+    captured into a graph (it raises): lr and the step count are numbers of the host."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096, seed=0):
         if state_bits not in (32, 8):
