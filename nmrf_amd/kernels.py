@@ -1493,7 +1493,8 @@ ADAMW_BLOCK, GRAD_SQSUM_CHUNK = 256, 8192
 
 
 def _raw_stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())            # (torch.cuda.current_stream() builds an object: 2.5 us)
+    # (torch.cuda.current_stream() builds an object: 2.5 us; torch.cuda.current_device() asks whether CUDA is up, which the call's tensors show)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def adamw_step(n, p, g, m, v, m_scale, v_scale, numel, hyper, key, betas, dtype, state_bits, grad_scale):

@@ -9,11 +9,15 @@ from torch.autograd.function import once_differentiable
 from .. import kernels as K
 from .._lib import NmrfHipError
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 _GATE_ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
 
 
 def check_rows(name, names, tensors):
-    """One device, one type of fp32 / bf16 / fp16, on the GPU."""
+    """One device, one type of fp32 / bf16 / fp16, on the GPU; and no recording by operations (make_fx), which goes inside a Function and would hold
+    nothing of the kernels but the allocation of their outputs."""
+    if torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise NmrfHipError("%s is not recorded by make_fx (torch.jit.trace holds it as one call)" % name)
     ref = tensors[0]
     dtype, device = ref.dtype, ref.device
     if not ref.is_cuda:

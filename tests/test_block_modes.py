@@ -7,7 +7,9 @@ import ctypes
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
+from nmrf_amd import _lib
 from nmrf_amd.ops import blocks
 
 pytestmark = pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
@@ -104,6 +106,22 @@ def test_outputs_may_be_changed_in_place(by_address):
         for o in outputs(f(*args)):
             o += 1.0
             assert o.requires_grad
+
+
+def recordings_are_refused(device):
+    for leaf in (False, True):
+        for f, args in calls(device, leaf=leaf):
+            with pytest.raises(_lib.NmrfHipError, match="make_fx"):
+                make_fx(f)(*args)
+
+
+def test_recording_by_operations_is_refused():
+    recordings_are_refused("cpu")
+
+
+@pytest.mark.gpu
+def test_recording_by_operations_is_refused_on_the_device():
+    recordings_are_refused("cuda")
 
 
 @pytest.mark.gpu
